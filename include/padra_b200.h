@@ -320,6 +320,80 @@ PADRA_API int padra_exl3_moe_decode_layer_static(const padra_matrix *matrices, i
                                                  padra_stream stream);
 
 
+/* ---- the attention half of the layer: norm and rotation, the paged 4-bit cache, attention over it -----------------
+ * The experts' callers need these on this GPU too; the reference's own kernels for them (src/cuda/qk_rope_*, kv_*,
+ * attention_*) refuse it and know neither pages nor a 4-bit cache.  The structs below are read on the host during the
+ * call; the arrays they point to are device memory, read in stream order.
+ *
+ * Cache: pool[pages][kv_heads] blocks of page_size * (head_dim + head_dim / 8) bytes, each
+ *   K codes [page_size][head_dim / 2] | K scales FP16 [page_size][head_dim / 32] | V codes | V scales (as for K).
+ * Groups of 32 values share a scale s = FP16(max|x| / 7); code = clamp(rint(x / s), -7, 7) + 8 (8 where s is 0); the value is
+ * (code - 8) * s.  A row is head_dim / 8 little-endian words of eight codes, value i of the word's eight in bits [4i, 4i+4); word
+ * c * (head_dim / 32) + g holds values 32 g + 8 c .. + 7, so that a tensor-core lane finds its share of every group in one
+ * run of bytes.  4.5 bits per value.  head_dim 64 or 128, page_size a power of two in 16..256, pool 16-byte aligned.
+ *
+ * Sequences: sequence s of a call owns rows row_begin[s] .. row_begin[s+1]-1 of the row arrays (row_begin[0] = 0, at most
+ * max_rows of them), the last of which is at position context[s] - 1; its token p lives in page
+ * page_table[s * table_stride + p / page_size].  Rows from row_begin[count] up to `rows` belong to nobody and are left as they
+ * are; rows whose position would be negative (context shorter than the sequence's rows) are padding: nothing is appended
+ * for them and their attention is zero.  A page that a call appends to belongs to one sequence of that call; pages that
+ * are only read may be shared.  A page number outside the pool, a context beyond the table or row bounds that do not
+ * ascend within `rows` and max_rows raise *bad; what the call computes for that sequence is then unspecified, but nothing
+ * outside the described arrays is read or written.  A flag that is already raised is not looked at.
+ *
+ * Row arrays: [rows][heads][head_dim] with a stride per row in values (heads lie side by side, so columns of one
+ * projection's output can be passed); pointers 16-byte aligned, strides multiples of 8 values.  Types: BF16 or FP16 bit
+ * patterns, or FP32 (not for attention).  Sums, statistics and angles are held in 32 bits or more and the result is
+ * rounded once to the rows' type. */
+enum { PADRA_ROWS_BF16 = 0, PADRA_ROWS_F16 = 1, PADRA_ROWS_F32 = 2 };
+typedef struct padra_kv_cache {
+  void *pool;
+  long long pages;
+  int page_size, kv_heads, head_dim;
+} padra_kv_cache;
+typedef struct padra_sequences {
+  const int *page_table, *row_begin, *context;
+  int count, table_stride, rows, max_rows;
+} padra_sequences;
+/* Rotation of the first `dims` (a multiple of 16, 0..head_dim) values of a head: pair i turns by position * inv_freq[i] radians
+ * (inv_freq[dims / 2], FP64: any scaling for long contexts is in these numbers) and grows by `amplitude`.  Pairs are
+ * (x[i], x[i + dims / 2]), or (x[2i], x[2i + 1]) when interleaved.  Angles are reduced in 64 bits. */
+typedef struct padra_rotary {
+  const double *inv_freq;
+  double amplitude;
+  int dims, interleaved;
+} padra_rotary;
+
+/* Per head: y = x * weight / sqrt(mean(x^2) + eps) (weight BF16 bits [head_dim]; NULL: no norm), then the rotation at
+ * positions[row] (rotary NULL or dims 0: none).  q [rows][q_heads], k [rows][k_heads] in one launch (k_heads 0: only q); in
+ * place allowed.  head_dim 64, 128 or 256.  A result that is not finite in the rows' type raises *bad. */
+PADRA_API int padra_qk_norm_rope(const void *q, void *q_out, long long q_stride, long long q_out_stride, int q_heads,
+                                 const void *k, void *k_out, long long k_stride, long long k_out_stride, int k_heads,
+                                 const unsigned short *q_weight, const unsigned short *k_weight, double eps,
+                                 const int *positions, const padra_rotary *rotary, int rows, int head_dim, int type,
+                                 int *bad, padra_stream stream);
+/* Appends the rows' K (normed with k_weight unless NULL, rotated unless rotary is NULL) and V to the cache, and, when q is
+ * given, writes the rows' normed and rotated Q to q_out in the same launch.  K is normed and rotated in 64 bits and not
+ * rounded before it becomes codes, so the cache's bytes depend on the inputs alone and not on batch or launch shape.
+ * A K or V head with a value that is not finite or above 57344 in magnitude (where FP16 values of the codes end) raises
+ * *bad and is not written. */
+PADRA_API int padra_kv_append(const padra_kv_cache *cache, const padra_sequences *sequences, const void *k, const void *v,
+                              long long k_stride, long long v_stride, const unsigned short *k_weight, double eps,
+                              const padra_rotary *rotary, const void *q, void *q_out, long long q_stride,
+                              long long q_out_stride, int q_heads, const unsigned short *q_weight, int type, int *bad,
+                              padra_stream stream);
+/* Writes the values of the sequences' cached tokens at their rows' positions (row_begin / context as for append: with
+ * as many rows as context, whole sequences) to k_out and v_out. */
+PADRA_API int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *sequences, void *k_out, void *v_out,
+                            long long k_stride, long long v_stride, int type, int *bad, padra_stream stream);
+/* out = softmax(scale * q k^T) v over the cache: row at position p attends to tokens t <= p, with window > 0 only to
+ * t > p - window.  q, out [rows][q_heads], q_heads a multiple of the cache's kv_heads (heads g * q_heads / kv_heads .. share KV
+ * head g); out may not overlap q.  Call after the rows' own K and V have been appended.  A query that is not finite raises
+ * *bad and gives zeros. */
+PADRA_API int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out,
+                                 long long q_stride, long long out_stride, int q_heads, int type, float scale,
+                                 int window, int *bad, padra_stream stream);
+
 /* ---- utilities ------------------------------------------------------------------------------------------
  * Full FP16 decode of one matrix through the same codec the kernels use: out[input*rows + output].
  * `matrix` is a device pointer to one descriptor.  For verification; not on the timed path.

@@ -1,0 +1,155 @@
+"""The attention half of a decoder layer: per-head norm and rotation, the paged 4-bit cache, attention over it.
+
+Python-side callers of padra_qk_norm_rope, padra_kv_append, padra_kv_read and padra_attention_q4 (formulas, cache format and
+contracts: include/padra_b200.h).  `KvCache` owns one layer's pool, `Sequences` describes the rows of a call, `Rotary` the position
+rotation; `AttentionKernels` passes their pointers through.  The reference's counterparts are its attention_*, kv_* and
+qk_rope_* kernels (src/cuda/), which neither run on this GPU nor know pages or a 4-bit cache.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import binding as B
+
+GROUP = 32  # values that share an FP16 scale
+ROWS_TYPE = {torch.bfloat16: B.ROWS_BF16, torch.float16: B.ROWS_F16, torch.float32: B.ROWS_F32}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+class KvCache:
+    """One layer's cache: `pages` pages of `page_size` tokens for `kv_heads` KV heads, 4.5 bits per value."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda"):
+        _need(head_dim in (64, 128), "head_dim is 64 or 128")
+        self._set(torch.zeros((pages, kv_heads, self.block_bytes(page_size, head_dim)), dtype=torch.uint8, device=device), page_size, head_dim)
+
+    @staticmethod
+    def block_bytes(page_size: int, head_dim: int) -> int:
+        """Bytes of one page of one KV head."""
+        return page_size * (head_dim + head_dim // 8)
+
+    @classmethod
+    def over(cls, pool: torch.Tensor, page_size: int, head_dim: int) -> "KvCache":
+        """A cache in memory that the caller has: pool [pages][kv_heads][block bytes], uint8."""
+        self = cls.__new__(cls)
+        self._set(pool, page_size, head_dim)
+        return self
+
+    def _set(self, pool, page_size, head_dim):
+        _need(pool.dtype == torch.uint8 and pool.dim() == 3 and pool.is_contiguous() and pool.shape[2] == self.block_bytes(page_size, head_dim),
+              "pool is a contiguous uint8 tensor [pages][kv_heads][block bytes]")
+        self.pool, self.page_size, self.head_dim = pool, page_size, head_dim
+        self.pages, self.kv_heads = pool.shape[:2]
+        self.struct = B.KvCacheStruct(pool.data_ptr(), self.pages, page_size, self.kv_heads, head_dim)
+        self.ref = C.addressof(self.struct)
+
+
+class Sequences:
+    """Whose rows a call works on: page_table [count][stride], row_begin [count + 1], context [count], all int32 on the device.
+    `rows` is the number of rows of the row arrays, `max_rows` the most that one sequence has; both are known on the host,
+    so that nothing has to be read back and a captured call can be replayed with new contents of the three tensors."""
+
+    def __init__(self, page_table: torch.Tensor, row_begin: torch.Tensor, context: torch.Tensor, rows: int, max_rows: int):
+        count = context.numel()
+        for t in (page_table, row_begin, context):
+            _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == context.device, "page_table, row_begin and context are contiguous int32 tensors of one device")
+        _need(page_table.dim() == 2 and page_table.shape[0] == count and row_begin.numel() == count + 1, "page_table [count][stride], row_begin [count + 1], context [count]")
+        self.page_table, self.row_begin, self.context, self.rows, self.max_rows = page_table, row_begin, context, rows, max_rows
+        self.struct = B.SequencesStruct(page_table.data_ptr(), row_begin.data_ptr(), context.data_ptr(), count, page_table.shape[1], rows, max_rows)
+        self.ref = C.addressof(self.struct)
+
+
+class Rotary:
+    """Rotation of the first 2 * len(inv_freq) values of a head; inv_freq (float64, device) in radians per position."""
+
+    def __init__(self, inv_freq: torch.Tensor, interleaved: bool = False, amplitude: float = 1.0):
+        _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq is a contiguous float64 vector")
+        self.inv_freq = inv_freq
+        self.struct = B.RotaryStruct(inv_freq.data_ptr(), amplitude, 2 * inv_freq.numel(), int(interleaved))
+        self.ref = C.addressof(self.struct)
+
+
+def _heads(x: torch.Tensor, what: str) -> int:
+    """Row stride of a [rows][heads][head_dim] tensor whose heads lie side by side."""
+    heads, dim = x.shape[1:]
+    stride = x.stride()
+    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
+        raise ValueError(f"{what}: heads of a row lie side by side")
+    return stride[0] if x.shape[0] > 1 else heads * dim
+
+
+class AttentionKernels:
+    """Callers of the C ABI on the current stream (or `stream`) of the current device."""
+
+    def __init__(self, device="cuda"):
+        self.lib = B.load()
+        self.bad = torch.zeros(1, dtype=torch.int32, device=device)
+        self._bad = self.bad.data_ptr()
+
+    def reset_bad(self):
+        self.bad.zero_()
+
+    def bad_flag(self) -> int:
+        return int(self.bad.item())
+
+    @staticmethod
+    def _weight(w, dim):
+        if w is None:
+            return None
+        _need(w.dtype in (torch.bfloat16, torch.uint16) and w.numel() == dim and w.is_contiguous(), "norm weights are BF16 vectors of head_dim values")
+        return w.data_ptr()
+
+    def qk_norm_rope(self, q, k, positions, rotary=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None, stream=None):
+        """Per-head RMS norm (where a weight is given) and rotation of q and k (k may be None); returns (q_out, k_out)."""
+        rows, q_heads, dim = q.shape
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+        _need(q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out is shaped and typed as q")
+        _need(positions is None or (positions.dtype == torch.int32 and positions.numel() == rows and positions.is_contiguous()), "positions: int32 [rows]")
+        k_args = (None, None, 0, 0, 0)
+        if k is not None:
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
+            _need(k.shape[::2] == (rows, dim) and k.dtype == q.dtype and k_out.shape == k.shape and k_out.dtype == k.dtype, "k and k_out: rows, head size and type of q")
+            k_args = (k.data_ptr(), k_out.data_ptr(), _heads(k, "k"), _heads(k_out, "k_out"), k.shape[1])
+        B.check(self.lib.padra_qk_norm_rope(q.data_ptr(), q_out.data_ptr(), _heads(q, "q"), _heads(q_out, "q_out"), q_heads, *k_args,
+                                            self._weight(q_weight, dim), self._weight(k_weight, dim), eps, B.ptr(positions),
+                                            rotary and rotary.ref, rows, dim, ROWS_TYPE[q.dtype], self._bad, B.stream_handle(stream)),
+                "padra_qk_norm_rope")
+        return q_out, k_out
+
+    def append(self, cache, sequences, k, v, rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None, q_out=None, stream=None):
+        """Appends the rows' K (normed, rotated) and V; with q also norms and rotates the rows' queries and returns them."""
+        dim, shape = cache.head_dim, (sequences.rows, cache.kv_heads, cache.head_dim)
+        _need(k.shape == shape and v.shape == shape and v.dtype == k.dtype, "k and v are [rows][kv_heads][head_dim] of one type")
+        q_args = (None, None, 0, 0, 0, None)
+        if q is not None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+            _need(q.shape[::2] == shape[::2] and q.dtype == k.dtype and q_out.shape == q.shape and q_out.dtype == q.dtype, "q and q_out: rows, head size and type of k")
+            q_args = (q.data_ptr(), q_out.data_ptr(), _heads(q, "q"), _heads(q_out, "q_out"), q.shape[1], self._weight(q_weight, dim))
+        B.check(self.lib.padra_kv_append(cache.ref, sequences.ref, k.data_ptr(), v.data_ptr(), _heads(k, "k"), _heads(v, "v"),
+                                         self._weight(k_weight, dim), eps, rotary and rotary.ref, *q_args, ROWS_TYPE[k.dtype], self._bad,
+                                         B.stream_handle(stream)), "padra_kv_append")
+        return q_out
+
+    def read(self, cache, sequences, k_out=None, v_out=None, dtype=torch.bfloat16, stream=None):
+        """The values of the cached tokens at the rows' positions; returns (k_out, v_out)."""
+        shape = (sequences.rows, cache.kv_heads, cache.head_dim)
+        k_out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if k_out is None else k_out
+        v_out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if v_out is None else v_out
+        _need(k_out.shape == shape and v_out.shape == shape and v_out.dtype == k_out.dtype, "k_out and v_out are [rows][kv_heads][head_dim] of one type")
+        B.check(self.lib.padra_kv_read(cache.ref, sequences.ref, k_out.data_ptr(), v_out.data_ptr(), _heads(k_out, "k_out"), _heads(v_out, "v_out"),
+                                       ROWS_TYPE[k_out.dtype], self._bad, B.stream_handle(stream)), "padra_kv_read")
+        return k_out, v_out
+
+    def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
+        """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+        _need(q.shape[::2] == (sequences.rows, cache.head_dim) and out.shape == q.shape and out.dtype == q.dtype, "q and out are [rows][heads][head_dim] of one type")
+        B.check(self.lib.padra_attention_q4(cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _heads(q, "q"), _heads(out, "out"), q.shape[1],
+                                            ROWS_TYPE[q.dtype], scale, window, self._bad, B.stream_handle(stream)), "padra_attention_q4")
+        return out

@@ -15,8 +15,11 @@ OK, INVALID_ARGUMENT, UNSUPPORTED, RESOURCE_EXHAUSTED, INTERNAL = 0, 1, 5, 6, 8
 FORMAT_OF_RATE = {3: 6, 4: 3, 6: 5}  # reference: src/cuda/device_matrix.cuh:30-44
 MAX_DECODE_ROWS = 16
 
+ROWS_BF16, ROWS_F16, ROWS_F32 = 0, 1, 2  # types of the attention path's row arrays
+
 _p = C.c_void_p
 _i = C.c_int
+_l = C.c_longlong
 
 # name -> argument types, in the order of include/padra_b200.h
 SIGNATURES = {
@@ -60,8 +63,24 @@ SIGNATURES = {
     "padra_route_group_schedule": ([_p, _p, _p, _p, _p, _p, _p, _i, _p, _p, _p], _i),
     "padra_residual_norm": ([_p, _p, _p, _p, _i, _i, _p, _p, _p], _i),
     "padra_combine_norm": ([_p, _p, _p, _p, _p, _i, _i, _p, _p, _p], _i),
+    "padra_qk_norm_rope": ([_p, _p, _l, _l, _i, _p, _p, _l, _l, _i, _p, _p, C.c_double, _p, _p, _i, _i, _i, _p, _p], _i),
+    "padra_kv_append": ([_p, _p, _p, _p, _l, _l, _p, C.c_double, _p, _p, _p, _l, _l, _i, _p, _i, _p, _p], _i),
+    "padra_kv_read": ([_p, _p, _p, _p, _l, _l, _i, _p, _p], _i),
+    "padra_attention_q4": ([_p, _p, _p, _p, _l, _l, _i, _i, C.c_float, _i, _p, _p], _i),
     "padra_codec_ceiling_launch": ([_i, _i, _i, _i, _p, _p], _i),
 }
+
+
+class KvCacheStruct(C.Structure):  # padra_kv_cache
+    _fields_ = [("pool", _p), ("pages", _l), ("page_size", _i), ("kv_heads", _i), ("head_dim", _i)]
+
+
+class SequencesStruct(C.Structure):  # padra_sequences
+    _fields_ = [("page_table", _p), ("row_begin", _p), ("context", _p), ("count", _i), ("table_stride", _i), ("rows", _i), ("max_rows", _i)]
+
+
+class RotaryStruct(C.Structure):  # padra_rotary
+    _fields_ = [("inv_freq", _p), ("amplitude", C.c_double), ("dims", _i), ("interleaved", _i)]
 
 
 class PadraError(RuntimeError):

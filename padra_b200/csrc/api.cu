@@ -313,4 +313,30 @@ int padra_exl3_decode_weights(const padra_matrix *matrix, unsigned short *out, i
   return LaunchDecodeWeights(matrix, out, rows, cols, rate, bad, S(stream));
 }
 
+int padra_qk_norm_rope(const void *q, void *q_out, long long q_stride, long long q_out_stride, int q_heads, const void *k, void *k_out,
+                       long long k_stride, long long k_out_stride, int k_heads, const unsigned short *q_weight,
+                       const unsigned short *k_weight, double eps, const int *positions, const padra_rotary *rotary, int rows, int head_dim,
+                       int type, int *bad, padra_stream stream) {
+  return LaunchNormRope(q, q_out, q_stride, q_out_stride, q_heads, k, k_out, k_stride, k_out_stride, k_heads, q_weight, k_weight, eps,
+                        positions, rotary, rows, head_dim, type, bad, S(stream));
+}
+
+int padra_kv_append(const padra_kv_cache *cache, const padra_sequences *sequences, const void *k, const void *v, long long k_stride,
+                    long long v_stride, const unsigned short *k_weight, double eps, const padra_rotary *rotary, const void *q, void *q_out,
+                    long long q_stride, long long q_out_stride, int q_heads, const unsigned short *q_weight, int type, int *bad,
+                    padra_stream stream) {
+  return LaunchKvAppend(cache, sequences, k, v, k_stride, v_stride, k_weight, eps, rotary, q, q_out, q_stride, q_out_stride, q_heads,
+                        q_weight, type, bad, S(stream));
+}
+
+int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *sequences, void *k_out, void *v_out, long long k_stride,
+                  long long v_stride, int type, int *bad, padra_stream stream) {
+  return LaunchKvRead(cache, sequences, k_out, v_out, k_stride, v_stride, type, bad, S(stream));
+}
+
+int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
+                       long long out_stride, int q_heads, int type, float scale, int window, int *bad, padra_stream stream) {
+  return LaunchAttention(cache, sequences, q, out, q_stride, out_stride, q_heads, type, scale, window, bad, S(stream));
+}
+
 } // extern "C"

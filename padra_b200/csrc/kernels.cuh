@@ -85,4 +85,18 @@ int LaunchPrefill(const Matrix *matrices, int layer, int part, const int *ids, c
                   const unsigned short *table, void *transformed, int tokens, int *bad, cudaStream_t stream, int rate,
                   int hidden, int inter);
 
+// The attention half of the layer (kv_cache.cu, attention.cu).
+int LaunchNormRope(const void *q, void *q_out, long long q_stride, long long q_out_stride, int q_heads, const void *k, void *k_out,
+                   long long k_stride, long long k_out_stride, int k_heads, const unsigned short *q_weight, const unsigned short *k_weight,
+                   double eps, const int *positions, const padra_rotary *rotary, int rows, int head_dim, int type, int *bad,
+                   cudaStream_t stream);
+int LaunchKvAppend(const padra_kv_cache *cache, const padra_sequences *sequences, const void *k, const void *v, long long k_stride,
+                   long long v_stride, const unsigned short *k_weight, double eps, const padra_rotary *rotary, const void *q, void *q_out,
+                   long long q_stride, long long q_out_stride, int q_heads, const unsigned short *q_weight, int type, int *bad,
+                   cudaStream_t stream);
+int LaunchKvRead(const padra_kv_cache *cache, const padra_sequences *sequences, void *k_out, void *v_out, long long k_stride, long long v_stride,
+                 int type, int *bad, cudaStream_t stream);
+int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
+                    long long out_stride, int q_heads, int type, float scale, int window, int *bad, cudaStream_t stream);
+
 } // namespace padra

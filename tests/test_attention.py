@@ -1,0 +1,414 @@
+"""Per-head norm and rotation, the paged 4-bit cache and attention over it, against the formulas in 64 bits
+(tests/attention_reference.py).  The refusals run on the CPU: they come from the C ABI's argument checks."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from tests import attention_reference as R
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}  # half a step, relative
+
+
+# ---- refusals (CPU) -------------------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def lib():
+    from padra_b200 import binding, build
+
+    build.build()
+    return binding.load()
+
+
+def structs(**over):
+    """Plausible structs over addresses that are never read."""
+    from padra_b200 import binding as B
+
+    c = dict(pool=4096, pages=4, page_size=16, kv_heads=2, head_dim=64)
+    s = dict(page_table=4096, row_begin=4096, context=4096, count=1, table_stride=2, rows=3, max_rows=3)
+    r = dict(inv_freq=4096, amplitude=1.0, dims=64, interleaved=0)
+    for k, v in over.items():
+        for d in (c, s, r):
+            if k in d:
+                d[k] = v
+    return B.KvCacheStruct(**c), B.SequencesStruct(**s), B.RotaryStruct(**r)
+
+
+@pytest.mark.parametrize("over, status", [
+    (dict(pool=4100), "INVALID_ARGUMENT"), (dict(pool=None), "INVALID_ARGUMENT"), (dict(pages=0), "INVALID_ARGUMENT"), (dict(pages=1 << 31), "INVALID_ARGUMENT"),
+    (dict(page_size=8), "INVALID_ARGUMENT"), (dict(page_size=48), "INVALID_ARGUMENT"), (dict(page_size=512), "INVALID_ARGUMENT"), (dict(kv_heads=0), "INVALID_ARGUMENT"),
+    (dict(head_dim=96), "UNSUPPORTED"), (dict(head_dim=256), "UNSUPPORTED"), (dict(count=-1), "INVALID_ARGUMENT"), (dict(rows=-1), "INVALID_ARGUMENT"),
+    (dict(table_stride=1 << 27), "INVALID_ARGUMENT"), (dict(row_begin=None), "INVALID_ARGUMENT"), (dict(page_table=None), "INVALID_ARGUMENT")])
+def test_cache_and_sequences_are_checked_before_anything_is_enqueued(lib, over, status):
+    from padra_b200 import binding as B
+
+    c, s, r = structs(**over)
+    want = getattr(B, status)
+    p = 4096
+    assert lib.padra_kv_append(C.byref(c), C.byref(s), p, p, 256, 256, None, 1e-6, None, None, None, 0, 0, 0, None, 0, p, None) == want
+    assert lib.padra_kv_read(C.byref(c), C.byref(s), p, p, 256, 256, 0, p, None) == want
+    assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None) == want
+
+
+def test_row_arguments_are_checked(lib):
+    from padra_b200 import binding as B
+
+    c, s, r = structs()
+    p = 4096
+    ok = [C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None]
+    for at, value, want in [(2, p + 2, B.INVALID_ARGUMENT), (2, None, B.INVALID_ARGUMENT), (3, p + 8, B.INVALID_ARGUMENT), (4, 255, B.INVALID_ARGUMENT),
+                            (4, 260, B.INVALID_ARGUMENT), (5, 128, B.INVALID_ARGUMENT), (6, 3, B.INVALID_ARGUMENT), (6, 0, B.INVALID_ARGUMENT),
+                            (7, B.ROWS_F32, B.UNSUPPORTED), (7, 9, B.UNSUPPORTED), (9, -1, B.INVALID_ARGUMENT), (10, None, B.INVALID_ARGUMENT)]:
+        args = list(ok)
+        args[at] = value
+        assert lib.padra_attention_q4(*args) == want, (at, value)
+    rope = [p, p, 256, 256, 4, None, None, 0, 0, 0, None, None, 1e-6, p, C.byref(r), 3, 64, 0, p, None]
+    for at, value, want in [(0, p + 4, B.INVALID_ARGUMENT), (2, 200, B.INVALID_ARGUMENT), (4, 0, B.INVALID_ARGUMENT), (9, 1, B.INVALID_ARGUMENT), (10, p + 2, B.INVALID_ARGUMENT),
+                            (12, -1.0, B.INVALID_ARGUMENT), (12, math.nan, B.INVALID_ARGUMENT), (13, None, B.INVALID_ARGUMENT), (16, 80, B.UNSUPPORTED), (17, 3, B.UNSUPPORTED), (18, None, B.INVALID_ARGUMENT)]:
+        args = list(rope)
+        args[at] = value
+        assert lib.padra_qk_norm_rope(*args) == want, (at, value)
+    for dims in (8, 24, 80, 128, -16):
+        _, _, bad = structs(dims=dims)
+        args = list(rope)
+        args[14] = C.byref(bad)
+        assert lib.padra_qk_norm_rope(*args) == B.INVALID_ARGUMENT, dims
+    append = [C.byref(c), C.byref(s), p, p, 128, 128, None, 1e-6, C.byref(r), p, p, 256, 256, 4, None, 0, p, None]
+    for at, value, want in [(2, p + 4, B.INVALID_ARGUMENT), (5, 120, B.INVALID_ARGUMENT), (10, None, B.INVALID_ARGUMENT), (13, 0, B.INVALID_ARGUMENT), (15, 5, B.UNSUPPORTED)]:
+        args = list(append)
+        args[at] = value
+        assert lib.padra_kv_append(*args) == want, (at, value)
+
+
+def test_nothing_to_do_is_not_an_error(lib):
+    from padra_b200 import binding as B
+
+    p = 4096
+    for over in (dict(rows=0), dict(count=0, row_begin=None, context=None)):
+        c, s, r = structs(**over)
+        assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None) == B.OK
+        assert lib.padra_kv_read(C.byref(c), C.byref(s), p, p, 128, 128, 0, p, None) == B.OK
+        assert lib.padra_kv_append(C.byref(c), C.byref(s), p, p, 128, 128, None, 1e-6, None, None, None, 0, 0, 0, None, 0, p, None) == B.OK
+    assert lib.padra_qk_norm_rope(p, p, 256, 256, 4, None, None, 0, 0, 0, None, None, 1e-6, p, None, 0, 64, 0, p, None) == B.OK
+
+
+def test_python_side_checks_shapes_and_types():
+    from padra_b200 import attention as A
+
+    with pytest.raises(ValueError):
+        A.KvCache(2, 16, 1, 96, device="cpu")
+    with pytest.raises(ValueError):
+        A.KvCache.over(torch.zeros((2, 1, 100), dtype=torch.uint8), 16, 64)
+    with pytest.raises(ValueError):
+        A.Rotary(torch.zeros(32))
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        A.Sequences(i[None], i, i, 4, 4)
+    with pytest.raises(ValueError):
+        A.Sequences(torch.zeros((3, 1), dtype=torch.int64), torch.zeros(4, dtype=torch.int32), i, 4, 4)
+
+
+def test_reference_quantiser_against_a_plain_loop():
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((2, 64), generator=g, dtype=torch.float64)
+    x[1, 32:] = 0
+    codes, scales = R.quantise(x)
+    for r in range(2):
+        for b in range(2):
+            most = max(abs(float(t)) for t in x[r, 32 * b:32 * b + 32])
+            s = float(torch.tensor(most / 7, dtype=torch.float64).to(torch.float16))
+            assert abs(float(scales[r, b]) - s) <= s * 2 ** -10
+            for d in range(32):
+                t = float(x[r, 32 * b + d])
+                assert int(codes[r, 32 * b + d]) == (round(t / float(scales[r, b])) + 8 if s else 8)
+    pool = torch.zeros((1, 1, 16 * 72), dtype=torch.uint8)
+    R.store(pool, 0, 0, 5, 16, x[0], x[1])
+    k, v = R.fetch(pool, 0, 16, 64)
+    assert torch.equal(k[0, 5], R.dequantise(codes, scales)[0]) and torch.equal(v[0, 5], R.dequantise(codes, scales)[1])
+
+
+# ---- GPU ----------------------------------------------------------------------------------------------------------------
+
+class Call:
+    """A pool, a page table in random order and rows for ragged sequences, on both sides."""
+
+    def __init__(self, gpu, shapes, heads, kv_heads, dim, page, dtype, seed, spare_rows=0, spare_pages=2, strided=True):
+        from padra_b200 import attention as A
+
+        g = self.g = torch.Generator().manual_seed(seed)
+        self.shapes, self.heads, self.kv_heads, self.dim, self.page, self.dtype, self.gpu = shapes, heads, kv_heads, dim, page, dtype, gpu
+        need = [-(-c // page) for _, c in shapes]
+        pages = sum(need) + spare_pages
+        order = torch.randperm(pages, generator=g)
+        self.table = torch.full((len(shapes), max(need + [1])), -1, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = order[at:at + n]
+            at += n
+        self.begin = torch.tensor([0] + [n for n, _ in shapes], dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        self.context = torch.tensor([c for _, c in shapes], dtype=torch.int32)
+        self.rows = int(self.begin[-1]) + spare_rows
+        # anything a former user may have left in the pages, with finite scales
+        self.pool = torch.randint(0, 256, (pages, kv_heads, A.KvCache.block_bytes(page, dim)), generator=g, dtype=torch.uint8)
+        a, b = page * dim // 2, page * dim // 16
+        for at in (a, 2 * a + b):
+            n = pages * kv_heads * page * dim // 32
+            self.pool[:, :, at:at + b] = (torch.rand(n, generator=g) * 0.4).to(torch.float16).view(torch.uint8).view(pages, kv_heads, b)
+        width = (heads + 2 * kv_heads) * dim + (16 if strided else 0)
+        self.qkv = torch.randn((self.rows, width), generator=g).to(dtype)
+        self.split()
+        self.kernels = A.AttentionKernels(gpu)
+        self.cache = A.KvCache.over(self.pool.to(gpu), page, dim)
+        self.d_qkv = self.qkv.to(gpu)
+        self.dq, self.dk, self.dv = self.views(self.d_qkv)
+        self.sequences = A.Sequences(self.table.to(gpu), self.begin.to(gpu), self.context.to(gpu), self.rows, max([n for n, _ in shapes] + [0]))
+
+    def views(self, qkv):
+        h, kv, d = self.heads, self.kv_heads, self.dim
+        return (qkv[:, :h * d].unflatten(1, (h, d)), qkv[:, h * d:(h + kv) * d].unflatten(1, (kv, d)), qkv[:, (h + kv) * d:(h + 2 * kv) * d].unflatten(1, (kv, d)))
+
+    def split(self):
+        self.q, self.k, self.v = self.views(self.qkv)
+
+    def reference(self, scale, window, pool=None):
+        pool = self.pool if pool is None else pool
+        want, bound = torch.zeros((self.rows, self.heads, self.dim), dtype=torch.float64), torch.zeros((self.rows, self.heads, self.dim), dtype=torch.float64)
+        for s, (n, c) in enumerate(self.shapes):
+            b = int(self.begin[s])
+            k, v = R.tokens(pool, self.table[s], c, self.page, self.dim)
+            want[b:b + n], bound[b:b + n] = R.attention(self.q[b:b + n], k, v, c - n, scale, window)
+        return want, bound
+
+    def check_attention(self, scale=None, window=0, what="attention"):
+        scale = self.dim ** -0.5 if scale is None else scale
+        out = torch.full((self.rows, self.heads, self.dim), 7.0, dtype=self.dtype, device=self.gpu)
+        self.kernels.attention(self.cache, self.sequences, self.dq, scale, window, out)
+        assert self.kernels.bad_flag() == 0
+        got, last = out.cpu().double(), int(self.begin[-1])
+        want, bound = self.reference(scale, window)
+        assert (got[last:] == 7).all(), "rows behind the last sequence were touched"
+        off = (got[:last] - want[:last]).abs() - (bound[:last] + HALF[self.dtype] * want[:last].abs() + 1e-7)
+        assert off.max().item() <= 0 if off.numel() else True, f"{what}: {off.max().item():.3e} beyond the bound"
+        return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows, heads, kv_heads, dim, dims, interleaved, norm", [
+    (1, 1, 1, 64, 64, False, True), (1, 32, 4, 128, 128, False, True), (3, 5, 3, 64, 32, True, True), (7, 7, 1, 128, 64, False, False),
+    (601, 4, 2, 64, 16, True, True), (1203, 3, 1, 256, 256, False, True), (33, 2, 2, 256, 48, True, False), (5, 4, 0, 128, 0, False, True)])
+def test_norm_and_rotation(gpu, dtype, rows, heads, kv_heads, dim, dims, interleaved, norm):
+    from padra_b200 import attention as A
+
+    g = torch.Generator().manual_seed(rows + dim)
+    qkv = (torch.randn((rows, heads + kv_heads + 1, dim), generator=g) * torch.exp(torch.randn((rows, 1, 1), generator=g))).to(dtype)
+    q, k = qkv[:, :heads], qkv[:, heads:heads + kv_heads] if kv_heads else None
+    weights = [(1 + 0.3 * torch.randn(dim, generator=g)).bfloat16() if norm else None for _ in range(2)]
+    positions = torch.randint(0, 1 << 17, (rows,), generator=g, dtype=torch.int32)
+    positions[0] = 0
+    inv_freq, amplitude = R.yarn_like(dims // 2, 4.0) if dims else (torch.zeros(0, dtype=torch.float64), 1.0)
+    kernels = A.AttentionKernels(gpu)
+    rotary = A.Rotary(inv_freq.to(gpu), interleaved, amplitude) if dims else None
+    d = qkv.to(gpu)
+    got = kernels.qk_norm_rope(d[:, :heads], d[:, heads:heads + kv_heads] if kv_heads else None, positions.to(gpu), rotary,
+                               *[None if w is None else w.to(gpu) for w in weights], 1e-6)
+    assert kernels.bad_flag() == 0
+    for x, w, y in zip((q, k), weights, got):
+        if x is None:
+            continue
+        normed = R.rms(x, w, 1e-6)
+        want = R.rotate(normed, positions, inv_freq, interleaved, amplitude)
+        # FP32 on the way: the norm's factor is off by about 14 * 2^-24, products, the reduced angle (2^-22) and sincos (2^-23) add
+        # up to less than 2^-19 of the pair's two values
+        slack = 2.0 ** -19 * 2 * amplitude * normed.abs().amax(-1, keepdim=True)
+        assert ((y.cpu().double() - want).abs() <= HALF[dtype] * want.abs() + slack).all()
+    # in place, and the same bits
+    kernels.qk_norm_rope(d[:, :heads], d[:, heads:heads + kv_heads] if kv_heads else None, positions.to(gpu), rotary,
+                         *[None if w is None else w.to(gpu) for w in weights], 1e-6, d[:, :heads], d[:, heads:heads + kv_heads] if kv_heads else None)
+    assert torch.equal(d[:, :heads], got[0]) and (not kv_heads or torch.equal(d[:, heads:heads + kv_heads], got[1]))
+    assert torch.equal(d[:, -1].cpu(), qkv[:, -1])
+
+
+@pytest.mark.gpu
+def test_norm_and_rotation_report_what_is_not_finite(gpu):
+    from padra_b200 import attention as A
+
+    kernels = A.AttentionKernels(gpu)
+    x = torch.ones((2, 1, 64), dtype=torch.float16, device=gpu)
+    kernels.qk_norm_rope(x, None, None)
+    assert kernels.bad_flag() == 0
+    x[1, 0, 3] = float("inf")
+    kernels.qk_norm_rope(x, None, None)
+    assert kernels.bad_flag() == 1
+
+
+SHAPES = {
+    "one": [(1, 1)], "decode": [(1, 130), (1, 1), (1, 64), (1, 17)], "verify": [(5, 40), (2, 2), (16, 333)],
+    "empty": [(0, 0), (1, 33), (0, 20), (3, 3), (0, 0)], "padded": [(4, 2), (1, 0), (3, 3)], "chunk": [(70, 200), (129, 129), (1, 300)]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", SHAPES)
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim, page, dims, interleaved, norm", [
+    (torch.bfloat16, 8, 2, 128, 64, 128, False, True), (torch.float16, 3, 3, 64, 16, 32, True, True), (torch.float32, 4, 1, 64, 128, 64, False, False),
+    (torch.bfloat16, 5, 5, 128, 32, 0, False, True)])
+def test_append_writes_the_bytes_of_the_definition(gpu, shapes, dtype, heads, kv_heads, dim, page, dims, interleaved, norm):
+    from padra_b200 import attention as A
+
+    c = Call(gpu, SHAPES[shapes], heads, kv_heads, dim, page, dtype, 11, spare_rows=3)
+    c.v[0, 0, :32] = 0  # a group of zeros
+    if dtype != torch.float16:
+        c.v[0, 0, 32:64] = torch.tensor([3.5, -2.5, 1.5, 0.5, 7.0, -7.0, 6.5, 5.5] * 4).to(dtype)  # scale 1: values on the borders
+    c.d_qkv.copy_(c.qkv)
+    weights = [(1 + 0.3 * torch.randn(dim, generator=c.g)).bfloat16() if norm else None for _ in range(2)]
+    inv_freq, amplitude = R.yarn_like(dims // 2, 2.0) if dims else (torch.zeros(0, dtype=torch.float64), 1.0)
+    rotary = A.Rotary(inv_freq.to(gpu), interleaved, amplitude) if dims else None
+    dw = [None if w is None else w.to(gpu) for w in weights]
+    q_out = torch.full((c.rows, heads, dim), 7.0, dtype=dtype, device=gpu)
+    c.kernels.append(c.cache, c.sequences, c.dk, c.dv, rotary, dw[1], 1e-6, c.dq, dw[0], q_out)
+    assert c.kernels.bad_flag() == 0
+    want = c.pool.clone()
+    q_want, q_there = torch.full((c.rows, heads, dim), 7.0, dtype=torch.float64), torch.zeros(c.rows, dtype=torch.bool)
+    for s, (n, ctx) in enumerate(c.shapes):
+        b = int(c.begin[s])
+        at = torch.arange(ctx - n, ctx)
+        k = R.rotate(R.rms(c.k[b:b + n], weights[1], 1e-6), at, inv_freq, interleaved, amplitude)
+        q_want[b:b + n] = R.rotate(R.rms(c.q[b:b + n], weights[0], 1e-6), at, inv_freq, interleaved, amplitude)
+        for r in range(n):
+            p = ctx - n + r
+            q_there[b + r] = p >= 0
+            for h in range(kv_heads if p >= 0 else 0):
+                R.store(want, int(c.table[s, p // page]), h, p % page, page, k[r, h], c.v[b + r, h].double())
+    assert torch.equal(c.cache.pool.cpu(), want)
+    got = q_out.cpu().double()
+    assert (got[~q_there] == 7).all()
+    slack = 2.0 ** -19 * 2 * amplitude * q_want.abs().amax(-1, keepdim=True) * math.sqrt(2)
+    assert ((got - q_want).abs() <= HALF[dtype] * q_want.abs() + slack)[q_there].all()
+    # and back
+    k_back, v_back = (torch.full((c.rows, kv_heads, dim), 7.0, dtype=torch.float32, device=gpu) for _ in range(2))
+    c.kernels.read(c.cache, c.sequences, k_back, v_back)
+    assert (k_back.cpu()[~q_there] == 7).all()
+    for s, (n, ctx) in enumerate(c.shapes):
+        k, v = R.tokens(want, c.table[s], ctx, page, dim)
+        b, skip = int(c.begin[s]), max(0, n - ctx)
+        assert torch.equal(k_back.cpu()[b + skip:b + n].double(), k[ctx - n + skip:]) and torch.equal(v_back.cpu()[b + skip:b + n].double(), v[ctx - n + skip:])
+    k16, v16 = c.kernels.read(c.cache, c.sequences, dtype=torch.bfloat16)
+    assert torch.equal(k16[q_there], k_back[q_there].bfloat16()) and torch.equal(v16[q_there], v_back[q_there].bfloat16())
+    assert c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 60000.0])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_append_leaves_out_a_head_that_four_bits_cannot_hold(gpu, value, which):
+    c = Call(gpu, [(2, 5), (1, 9)], 4, 2, 64, 16, torch.float32, 5)
+    getattr(c, which)[1, 1, 40] = value
+    c.d_qkv.copy_(c.qkv)
+    c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
+    assert c.kernels.bad_flag() == 1
+    want = c.pool.clone()
+    for s, (n, ctx) in enumerate(c.shapes):
+        for r in range(n):
+            b, p = int(c.begin[s]) + r, ctx - n + r
+            for h in range(2):
+                page, slot = int(c.table[s, p // 16]), p % 16
+                before = R.fetch(want, page, 16, 64)
+                k, v = c.k[b, h].double(), c.v[b, h].double()
+                if (b, h) == (1, 1):
+                    k, v = (before[0][h, slot], v) if which == "k" else (k, before[1][h, slot])
+                R.store(want, page, h, slot, 16, k, v)
+    got, held = c.cache.pool.cpu(), c.pool
+    page, slot = int(c.table[0, 0]), 4
+    at = {"k": 0, "v": 16 * 36}[which] + slot * 32  # the head that was refused keeps its bytes
+    want[page, 1, at:at + 32] = held[page, 1, at:at + 32]
+    at = {"k": 0, "v": 16 * 36}[which] + 16 * 32 + slot * 4
+    want[page, 1, at:at + 4] = held[page, 1, at:at + 4]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(8, 2, 128, 64), (3, 3, 64, 16), (7, 1, 128, 16), (8, 1, 64, 128), (6, 2, 128, 256)])
+@pytest.mark.parametrize("shapes", SHAPES)
+@pytest.mark.parametrize("window", [0, 1, 50])
+def test_attention(gpu, dtype, heads, kv_heads, dim, page, shapes, window):
+    Call(gpu, SHAPES[shapes], heads, kv_heads, dim, page, dtype, 21, spare_rows=2).check_attention(window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_attention_with_other_scales(gpu, scale):
+    Call(gpu, [(1, 700), (3, 129), (40, 90)], 8, 2, 128, 64, torch.bfloat16, 23).check_attention(scale=scale)
+
+
+@pytest.mark.gpu
+def test_pages_that_do_not_exist_are_reported_and_not_read(gpu):
+    for page in (-1, 10 ** 6):
+        c = Call(gpu, [(1, 200), (40, 60), (1, 5)], 4, 2, 64, 16, torch.bfloat16, 31)
+        c.sequences.page_table[0, 3] = page
+        c.sequences.page_table[1, 1] = page
+        c.kernels.attention(c.cache, c.sequences, c.dq, 0.125)
+        assert c.kernels.bad_flag() == 1
+        c.kernels.reset_bad()
+        c.sequences.page_table[0, 12] = page  # the page that the last token goes to
+        c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
+        assert c.kernels.bad_flag() == 1
+        c.kernels.reset_bad()
+        c.kernels.read(c.cache, c.sequences)
+        assert c.kernels.bad_flag() == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fault", ["context beyond the table", "negative context", "rows beyond the array", "descending rows", "more rows than announced"])
+def test_contradicting_sequences_are_reported(gpu, fault):
+    c = Call(gpu, [(2, 40), (3, 60)], 4, 2, 64, 16, torch.bfloat16, 33)
+    s = c.sequences
+    if fault == "context beyond the table":
+        s.context[0] = 16 * s.page_table.shape[1] + 1
+    elif fault == "negative context":
+        s.context[1] = -5
+    elif fault == "rows beyond the array":
+        s.row_begin[2] = 60
+    elif fault == "descending rows":
+        s.row_begin[1] = -3
+    else:
+        s.struct.max_rows = 1
+    for call in (lambda: c.kernels.attention(c.cache, s, c.dq, 0.125), lambda: c.kernels.append(c.cache, s, c.dk, c.dv), lambda: c.kernels.read(c.cache, s)):
+        call()
+        assert c.kernels.bad_flag() == 1
+        c.kernels.reset_bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(1, 300), (1, 40)], [(40, 300), (1, 40)]])
+def test_queries_that_are_not_finite_are_reported_and_give_zeros(gpu, shapes):
+    c = Call(gpu, shapes, 4, 2, 64, 16, torch.bfloat16, 35)
+    good = c.check_attention()
+    c.dq[0, 1, 5] = float("nan")
+    c.dq[shapes[0][0], 3, 0] = float("-inf")
+    out = c.kernels.attention(c.cache, c.sequences, c.dq, 64 ** -0.5)
+    assert c.kernels.bad_flag() == 1
+    hurt = torch.zeros(out.shape[:2], dtype=torch.bool, device=gpu)
+    hurt[0, 1] = hurt[shapes[0][0], 3] = True
+    assert (out[hurt] == 0).all() and torch.equal(out[~hurt], good[~hurt])
+
+
+@pytest.mark.gpu
+def test_a_pool_of_more_than_four_gigabytes(gpu):
+    from padra_b200 import attention as A
+
+    c = Call(gpu, [(1, 200), (20, 90)], 8, 4, 128, 64, torch.bfloat16, 37)
+    pages = (5 << 30) // c.pool[0].numel()
+    pool = torch.empty((pages,) + c.pool.shape[1:], dtype=torch.uint8, device=gpu)
+    shift = pages - c.pool.shape[0]
+    pool[shift:] = c.pool.to(gpu)
+    pool[:c.pool.shape[0]] = 0
+    c.cache = A.KvCache.over(pool, 64, 128)
+    c.sequences.page_table += torch.where(c.sequences.page_table >= 0, shift, 0).int()
+    c.check_attention()
+    c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
+    back, _ = c.kernels.read(c.cache, c.sequences, dtype=torch.float32)
+    want = R.dequantise(*R.quantise(c.k.double()))
+    assert torch.equal(back.cpu().double(), want)
+    assert not pool[:c.pool.shape[0]].any() and c.kernels.bad_flag() == 0
