@@ -91,6 +91,7 @@ class AttentionKernels:
         self.lib = B.load()
         self.bad = torch.zeros(1, dtype=torch.int32, device=device)
         self._bad = self.bad.data_ptr()
+        self._workspace = {}  # (stream, head_dim) -> workspace: calls on one stream follow one another
 
     def reset_bad(self):
         self.bad.zero_()
@@ -146,10 +147,24 @@ class AttentionKernels:
                                        ROWS_TYPE[k_out.dtype], self._bad, B.stream_handle(stream)), "padra_kv_read")
         return k_out, v_out
 
+    def workspace(self, head_dim, stream):
+        """The workspace of calls on `stream` (a stream handle).  Made by the first call on the stream, which therefore comes
+        before any capture; captured calls keep using it, so graphs captured on one stream are not to be replayed side by side."""
+        key = stream, head_dim
+        if key not in self._workspace:
+            _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
+            n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
+            ws = torch.empty(n, dtype=torch.uint8, device=self.bad.device)
+            B.check(self.lib.padra_attention_q4_workspace_init(ws.data_ptr(), n, stream), "padra_attention_q4_workspace_init")
+            self._workspace[key] = ws, ws.data_ptr(), n
+        return self._workspace[key][1:]
+
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
         """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
         out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
         _need(q.shape[::2] == (sequences.rows, cache.head_dim) and out.shape == q.shape and out.dtype == q.dtype, "q and out are [rows][heads][head_dim] of one type")
+        handle = B.stream_handle(stream)
         B.check(self.lib.padra_attention_q4(cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _heads(q, "q"), _heads(out, "out"), q.shape[1],
-                                            ROWS_TYPE[q.dtype], scale, window, self._bad, B.stream_handle(stream)), "padra_attention_q4")
+                                            ROWS_TYPE[q.dtype], scale, window, *self.workspace(cache.head_dim, handle), self._bad, handle),
+                "padra_attention_q4")
         return out

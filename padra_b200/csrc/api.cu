@@ -334,9 +334,19 @@ int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *sequences,
   return LaunchKvRead(cache, sequences, k_out, v_out, k_stride, v_stride, type, bad, S(stream));
 }
 
+size_t padra_attention_q4_workspace_bytes(int head_dim) {
+  return AttentionWorkspaceBytes(head_dim);
+}
+
+int padra_attention_q4_workspace_init(void *workspace, size_t workspace_bytes, padra_stream stream) {
+  return InitAttentionWorkspace(workspace, workspace_bytes, S(stream));
+}
+
 int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
-                       long long out_stride, int q_heads, int type, float scale, int window, int *bad, padra_stream stream) {
-  return LaunchAttention(cache, sequences, q, out, q_stride, out_stride, q_heads, type, scale, window, bad, S(stream));
+                       long long out_stride, int q_heads, int type, float scale, int window, void *workspace, size_t workspace_bytes,
+                       int *bad, padra_stream stream) {
+  return LaunchAttention(cache, sequences, q, out, q_stride, out_stride, q_heads, type, scale, window, workspace, workspace_bytes, bad,
+                         S(stream));
 }
 
 } // extern "C"

@@ -1,122 +1,629 @@
-// Attention over the paged 4-bit cache: out = softmax(scale * q k^T + mask) v.
+// Attention over the paged 4-bit cache for few query rows per sequence: out = softmax(scale * q k^T + mask) v.
 //
-// One warp per (row, query head): 32 tokens at a time, one per lane for the scores, running maximum and sum, then every lane
-// gathers its share of the output over the 32 tokens.
+// With one row and G heads to a KV head there are G dot products per cached value: bound by the cache's bytes, if the codes
+// become tensor-core operands cheaply enough.
+//   * Work is (sequence, KV head, block of 8 * NT query columns) x 32-token tiles.  All tiles of a call form one list, and
+//     every CTA takes an equal run of it (ends may lie inside a sequence), so neither one long context nor ragged ones
+//     leave SMs idle.  A run's piece of a unit that is not the whole unit leaves maximum, sum and unnormalised output in the
+//     workspace; the CTA that arrives last at such a unit joins the pieces in list order, so results do not depend on
+//     timing.
+//   * A warp owns tiles w, w + 8, ... of the CTA's run, with a private ring of tiles filled by cp.async: no barrier between
+//     warps until the piece ends.
+//   * Scores: K is the MMA's A operand (16 tokens x 16 values), queries the B columns.  A lane's word holds eight codes of one
+//     group, and two MMAs cover a group of 32 values, so the FP16 scale of (token, group) is applied to the group's
+//     FP32 sum.  A code becomes an FP16 number by inserting it into the mantissa of 1024 (low nibble) or 64 (high nibble), one
+//     logic operation for two codes; the offsets (1032, 72) times the query are subtracted through the accumulator's
+//     initial value.
+//   * Output: V^T is the A operand (16 values x 16 tokens).  ldmatrix.trans on 16-bit pieces hands a lane four codes of two
+//     neighbouring tokens in one register, which is where the MMA wants a pair; offset and scale are applied as FP16 (codes
+//     and offsets exact, the product rounded once, 2^-12).  Weights go from the score layout to the B operand with one 8x8
+//     transpose (movmatrix) per eight tokens.
+//   * The running maximum is only raised when a weight would pass 2^15 (weights are FP16, at least 2^8 for the largest
+//     after a raise): a warp vote per tile instead of a reduction.
+#include <cmath>
+
 #include "kernels.cuh"
 #include "kv_cache.cuh"
 
 namespace padra {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kTile = 32;   // tokens of a tile
+constexpr int kStages = 5;  // tiles of a warp's ring
+constexpr int kMaxGrid = 1024; // CTAs the workspace provides for
+constexpr float kNever = -1e30f; // the running maximum before any token
+constexpr float kTop = 8.f, kRaise = 15.f; // log2 of the largest weight after a raise / before the next
 
-template <typename T> __device__ __forceinline__ float ToFloat(T x) { return static_cast<float>(x); }
-__device__ __forceinline__ void FromFloat(float x, __nv_bfloat16 *to) { *to = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void FromFloat(float x, __half *to) { *to = __float2half_rn(x); }
+struct AttentionArgs {
+  KvView cache;
+  SequenceView seq;
+  const void *q;
+  void *out;
+  long long q_stride, out_stride;
+  int q_heads, group; // heads that share a KV head
+  float scale;        // times log2(e)
+  int window;
+  float *partial;     // [grid][2][columns][head_dim + 2]
+  unsigned *ticket;   // [grid]: pieces of the split unit that begins in this CTA's run that have arrived
+  int *bad;
+};
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) AttentionKernel(KvView cache, SequenceView seq, const T *q, T *out, long long q_stride,
-                                                               long long out_stride, int q_heads, float scale, int window, int *bad) {
-  constexpr int kGroups = D / kKvGroup, kOwn = D / 32;
-  __shared__ float s_q[kWarps][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x, head = blockIdx.y * kWarps + warp, group = q_heads / cache.kv_heads;
-  if (head >= q_heads)
-    return;
-  int position = -1;
-  const int s = LocateRow(seq, cache, row, &position, bad);
-  if (s < 0)
-    return;
-  T *const mine = out + row * out_stride + head * D;
-  bool finite = true;
-  for (int d = lane; d < D; d += 32) {
-    const float x = position >= 0 ? ToFloat(q[row * q_stride + head * D + d]) : 0.f;
-    finite &= isfinite(x) != 0;
-    s_q[warp][d] = x * scale;
+__device__ __forceinline__ unsigned SmemAddress(const void *p) {
+  return static_cast<unsigned>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void CopyAsync16(unsigned to, const void *from, int bytes) { // the rest of the 16 bytes becomes zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void MmaF16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned Low(unsigned w) { // nibbles 0 and 4 as 1024 + n
+  return (w & 0x000f000fu) | 0x64006400u;
+}
+__device__ __forceinline__ unsigned High(unsigned w) { // nibbles 1 and 5 as 64 + n
+  return (w & 0x00f000f0u) | 0x54005400u;
+}
+__device__ __forceinline__ unsigned Scaled(unsigned x, unsigned offset, __half2 scale) {
+  const __half2 v = __hmul2(__hsub2(*reinterpret_cast<__half2 *>(&x), *reinterpret_cast<__half2 *>(&offset)), scale);
+  return *reinterpret_cast<const unsigned *>(&v);
+}
+__device__ __forceinline__ unsigned Pack(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned *>(&h);
+}
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void Load8(const __nv_bfloat16 *p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void Load8(const __half *p, float (&x)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+  const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
   }
-  if (__any_sync(0xffffffffu, !finite)) {
-    Raise(bad);
-    position = -1;
-  }
-  __syncwarp();
-  float m = -INFINITY, l = 0, o[kOwn] = {};
-  const int first = window > 0 && position >= window ? position - window + 1 : 0;
-  for (int t0 = first; t0 <= position; t0 += 32) {
-    const int t = t0 + lane;
-    float score = -INFINITY;
-    int page = -1;
-    if (t <= position)
-      page = PageOf(seq, cache, s, t, bad);
-    const int slot = t & (cache.page_size - 1);
-    const unsigned char *block = cache.block(page < 0 ? 0 : page, head / group);
-    if (page >= 0) {
-      score = 0;
-      for (int w = 0; w < D / 8; ++w) {
-        const int g = w % kGroups, c = w / kGroups;
-        const unsigned word = reinterpret_cast<const unsigned *>(block + slot * (D / 2))[w];
-        const float f = HalfBitsToFloat(reinterpret_cast<const unsigned short *>(block + cache.code_bytes() + slot * (D / 16))[g]);
-        float sum = 0;
-        for (int n = 0; n < 8; ++n)
-          sum += static_cast<float>(static_cast<int>(word >> (4 * n) & 15u) - 8) * s_q[warp][32 * g + 8 * c + n];
-        score += sum * f;
-      }
-    }
-    float most = score;
-    for (int d = 1; d < 32; d *= 2)
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-    if (most == -INFINITY)
-      continue;
-    const float next = fmaxf(m, most), shrink = expf(m - next), p = expf(score - next);
-    m = next, l = l * shrink;
-    for (int j = 0; j < kOwn; ++j)
-      o[j] *= shrink;
-    for (int n = 0; n < 32; ++n) {
-      const float pn = __shfl_sync(0xffffffffu, p, n);
-      const unsigned long long b = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(block), n);
-      const int sn = __shfl_sync(0xffffffffu, slot, n);
-      if (pn == 0.f)
-        continue;
-      l += pn;
-      const unsigned char *values = reinterpret_cast<const unsigned char *>(b) + cache.code_bytes() + cache.scale_bytes();
-      for (int j = 0; j < kOwn; ++j) {
-        const int d = j * 32 + lane, place = (d / 8 & 3) * kGroups + j;
-        const unsigned word = reinterpret_cast<const unsigned *>(values + sn * (D / 2))[place];
-        const float f = HalfBitsToFloat(reinterpret_cast<const unsigned short *>(values + cache.code_bytes() + sn * (D / 16))[j]);
-        o[j] += pn * f * static_cast<float>(static_cast<int>(word >> (4 * (d & 7)) & 15u) - 8);
-      }
-    }
-  }
-  for (int j = 0; j < kOwn; ++j)
-    FromFloat(l > 0 ? o[j] / l : 0.f, mine + j * 32 + lane);
+}
+__device__ __forceinline__ void Store4(__nv_bfloat16 *p, float4 v) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+  *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+}
+__device__ __forceinline__ void Store4(__half *p, float4 v) {
+  *reinterpret_cast<uint2 *>(p) = make_uint2(Pack(v.x, v.y), Pack(v.z, v.w));
 }
 
-template <typename T, int D>
-int Launch(const KvView &c, const SequenceView &s, const void *q, void *out, long long q_stride, long long out_stride, int q_heads, float scale,
-           int window, int *bad, cudaStream_t stream) {
-  AttentionKernel<T, D><<<dim3(s.rows, (q_heads + kWarps - 1) / kWarps), kWarps * 32, 0, stream>>>(
-      c, s, static_cast<const T *>(q), static_cast<T *>(out), q_stride, out_stride, q_heads, scale, window, bad);
+// What one sequence asks for: `blocks` column blocks of each KV head, `tiles` tiles for each of them, the first being tile
+// `first` of the sequence.  A sequence without rows, or one whose numbers contradict the call, has no work; rows that see
+// nothing still get one (empty) tile, so that their zeros are written.
+struct Demand {
+  int begin, rows, context, first, tiles, blocks;
+};
+template <int Columns> __device__ __forceinline__ Demand DemandOf(const AttentionArgs &a, int s) {
+  Demand d{};
+  if (!SequenceRows(a.seq, a.cache, s, &d.begin, &d.rows, &d.context, a.bad) || !d.rows)
+    return d;
+  const int low = a.window ? max(0, d.context - d.rows + 1 - a.window) : 0;
+  d.first = low / kTile;
+  d.tiles = max(1, (d.context + kTile - 1) / kTile - d.first);
+  d.blocks = (d.rows * a.group + Columns - 1) / Columns;
+  return d;
+}
+__device__ __forceinline__ long long CostOf(const AttentionArgs &a, const Demand &d) {
+  return static_cast<long long>(d.tiles) * d.blocks * a.cache.kv_heads;
+}
+
+template <int D> struct TileBytes {
+  static constexpr int kCodes = kTile * D / 2, kScales = kTile * D / 16, kAll = 2 * (kCodes + kScales);
+};
+
+// One piece: tiles [from, from + count) of a unit, `base` tiles into the sequence.
+template <typename T, int D, int NT> struct Piece {
+  static constexpr int kGroups = D / kKvGroup, kChunks = D / 32, kColumns = 8 * NT;
+  static constexpr int kRow = D + 4; // floats of a column's row in shared memory while warps are joined
+
+  // column -> row of the sequence and head of the group
+  static __device__ __forceinline__ void Run(const AttentionArgs &a, const Demand &d, int s, int head, int block, int first_tile, int count,
+                                             unsigned char *ring, float *join, float *join_ml) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const int columns = min(kColumns, d.rows * a.group - block * kColumns);
+    const int start = d.context - d.rows; // position of the sequence's first row
+
+    // ---- queries: FP16 after division by a power of two that brings the row's largest value below 2 ----
+    unsigned q[NT][kGroups][4];
+    float factor[NT][2], correction[NT][kGroups][2];
+    int last[NT][2], low[NT][2]; // tokens that columns 2c and 2c + 1 see
+    int least = 0x7fffffff, latest_low = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int column = 8 * n + g, place = block * kColumns + column, row = place / a.group, h = head * a.group + place % a.group;
+      float x[kGroups][8], most = 0;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        if (column < columns && start + row >= 0)
+          Load8(static_cast<const T *>(a.q) + static_cast<long long>(d.begin + row) * a.q_stride + h * D + 32 * i + 8 * c, x[i]);
+        else
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[i][j] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          finite &= isfinite(x[i][j]) != 0;
+          most = fmaxf(most, fabsf(x[i][j]));
+        }
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const bool fine = (__ballot_sync(0xffffffffu, !finite) & (0xfu << (lane & 28))) == 0;
+      if (!fine)
+        Raise(a.bad);
+      const int exponent = most > 0 && fine ? min(126, max(-126, ilogbf(most))) : 0;
+      const float shrink = fine ? ldexpf(1.f, -exponent) : 0.f;
+      float sums[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        float y[8], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[j] = fine ? __half2float(__float2half_rn(x[i][j] * shrink)) : 0.f;
+          sum += y[j] * (j & 1 ? -72.f : -1032.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q[n][i][j] = Pack(y[j], y[j + 4]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sums[i] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+      }
+      const float mine = a.scale * ldexpf(1.f, exponent);
+      // a row at a negative position sees nothing, nor does one that is not finite, nor a column beyond the last
+      const int to = column < columns && fine ? start + row : -1, from = a.window ? max(0, to - a.window + 1) : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int owner = 4 * (2 * c + e);
+        factor[n][e] = __shfl_sync(0xffffffffu, mine, owner);
+        last[n][e] = __shfl_sync(0xffffffffu, to, owner);
+        low[n][e] = __shfl_sync(0xffffffffu, from, owner);
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+          correction[n][i][e] = __shfl_sync(0xffffffffu, sums[i], owner);
+      }
+      if (column < columns)
+        least = min(least, to), latest_low = max(latest_low, from);
+    }
+#pragma unroll
+    for (int m = 4; m < 32; m *= 2) {
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
+      latest_low = max(latest_low, __shfl_xor_sync(0xffffffffu, latest_low, m));
+    }
+
+    float top[NT][2], sum[NT][2], o[NT][2 * kChunks][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n][0] = top[n][1] = kNever, sum[n][0] = sum[n][1] = 0;
+#pragma unroll
+      for (int t = 0; t < 2 * kChunks; ++t)
+        o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0;
+    }
+
+    // ---- the ring ----
+    const int mine = count > warp ? (count - warp + kWarps - 1) / kWarps : 0; // tiles of this warp: warp, warp + kWarps, ...
+    const int visible_low = a.window ? max(0, start + 1 - a.window) : 0;
+    unsigned char *const own_ring = ring + warp * kStages * TileBytes<D>::kAll;
+    const unsigned ring_address = SmemAddress(own_ring);
+    int page_low = -1, page_high = -1; // of this lane's tile among the next 32: first and second 16 tokens
+    auto fetch = [&](int i) {
+      if (i < mine) {
+        if ((i & 31) == 0) {
+          const int t = (first_tile + warp + (i + lane) * kWarps) * kTile;
+          page_low = page_high = -1;
+          if (i + lane < mine && t < d.context) {
+            if (a.cache.page_size > 16) {
+              page_low = page_high = PageOf(a.seq, a.cache, s, t, a.bad);
+            } else {
+              if (t + 16 > visible_low)
+                page_low = PageOf(a.seq, a.cache, s, t, a.bad);
+              if (t + 16 < d.context)
+                page_high = PageOf(a.seq, a.cache, s, t + 16, a.bad);
+            }
+          }
+        }
+        const int lo = __shfl_sync(0xffffffffu, page_low, i & 31), hi = __shfl_sync(0xffffffffu, page_high, i & 31);
+        const int t0 = (first_tile + warp + i * kWarps) * kTile;
+        const int slot = t0 & (a.cache.page_size - 1), shift_high = a.cache.page_size > 16 ? 0 : 16;
+        // first token of the tile in either page; a half without a page reads page 0's and gets scales of zero
+        const unsigned char *from_low = a.cache.block(max(lo, 0), head), *from_high = a.cache.block(max(hi, 0), head);
+        const unsigned to = ring_address + (i % kStages) * TileBytes<D>::kAll;
+        const int codes = a.cache.code_bytes(), scales = a.cache.scale_bytes();
+        constexpr int kRowsPerCopy = 32 / kChunks, kCopies = kTile / kRowsPerCopy; // tokens per warp-wide copy
+        const int token = lane / kChunks, chunk = lane % kChunks;
+        const int swizzled = kChunks == 4 ? chunk ^ ((token >> 1) & 3) : chunk ^ ((token >> 2) & 1);
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) {
+          const bool second = k * kRowsPerCopy >= 16;
+          const unsigned char *from = (second ? from_high - shift_high * (D / 2) : from_low) + (slot + k * kRowsPerCopy + token) * (D / 2) + 16 * chunk;
+          const unsigned at = to + (k * kRowsPerCopy + token) * (D / 2);
+          CopyAsync16(at + 16 * chunk, from, 16);
+          CopyAsync16(at + TileBytes<D>::kCodes + TileBytes<D>::kScales + 16 * swizzled, from + codes + scales, 16);
+        }
+        constexpr int kTokens = 256 / D, kLanes = kTile / kTokens; // tokens whose scales fit 16 bytes; lanes for K, as many for V
+        if (lane < 2 * kLanes) {
+          const int which = lane / kLanes, t = lane % kLanes * kTokens;
+          const bool second = t >= 16;
+          const int valid = (second ? hi : lo) < 0 ? 0 : max(0, min(kTokens, d.context - t0 - t));
+          const unsigned char *from = (second ? from_high - shift_high * (D / 16) : from_low) + codes + which * (codes + scales) + (slot + t) * (D / 16);
+          CopyAsync16(to + TileBytes<D>::kCodes + which * (TileBytes<D>::kCodes + TileBytes<D>::kScales) + t * (D / 16), from, valid * (D / 16));
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+      fetch(i);
+
+    for (int i = 0; i < mine; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp(); // the tile is here for every lane, and nobody reads the slot that is filled next
+      fetch(i + kStages - 1);
+      const unsigned char *const tile = own_ring + (i % kStages) * TileBytes<D>::kAll;
+      const int t0 = (first_tile + warp + i * kWarps) * kTile;
+      const bool edge = t0 + kTile - 1 > least || t0 < latest_low;
+
+      float score[2][NT][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        unsigned w[2][kGroups];
+        float f[2][kGroups];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int token = 16 * half + 8 * r + g;
+          if constexpr (kGroups == 4) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(tile + token * (D / 2) + 16 * c);
+            w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
+            const uint2 v = *reinterpret_cast<const uint2 *>(tile + TileBytes<D>::kCodes + token * (D / 16));
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+            f[r][0] = f0.x, f[r][1] = f0.y, f[r][2] = f1.x, f[r][3] = f1.y;
+          } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(tile + token * (D / 2) + 8 * c);
+            w[r][0] = u.x, w[r][1] = u.y;
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(tile + TileBytes<D>::kCodes + token * (D / 16)));
+            f[r][0] = f0.x, f[r][1] = f0.y;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          score[half][n][0] = score[half][n][1] = score[half][n][2] = score[half][n][3] = 0;
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+          const unsigned u0 = w[0][k], u1 = w[1][k], v0 = u0 >> 8, v1 = u1 >> 8;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float acc[4] = {correction[n][k][0], correction[n][k][1], correction[n][k][0], correction[n][k][1]};
+            MmaF16(acc, Low(u0), Low(u1), High(u0), High(u1), q[n][k][0], q[n][k][1]);
+            MmaF16(acc, Low(v0), Low(v1), High(v0), High(v1), q[n][k][2], q[n][k][3]);
+            score[half][n][0] += acc[0] * f[0][k], score[half][n][1] += acc[1] * f[0][k];
+            score[half][n][2] += acc[2] * f[1][k], score[half][n][3] += acc[3] * f[1][k];
+          }
+        }
+      }
+      // scores in units of log2, masked
+      float most = kNever;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = score[half][n][e] * factor[n][e & 1];
+            if (edge) {
+              const int t = t0 + 16 * half + 8 * (e >> 1) + g;
+              x = t > last[n][e & 1] || t < low[n][e & 1] ? -INFINITY : x;
+            }
+            score[half][n][e] = x;
+            most = fmaxf(most, x - top[n][e & 1]);
+          }
+      if (__any_sync(0xffffffffu, most > kRaise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = fmaxf(fmaxf(score[0][n][e], score[0][n][e + 2]), fmaxf(score[1][n][e], score[1][n][e + 2]));
+#pragma unroll
+            for (int m = 4; m < 32; m *= 2)
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+            const float next = fmaxf(top[n][e], x - kTop), shrink = Exp2(top[n][e] - next);
+            top[n][e] = next, sum[n][e] *= shrink;
+#pragma unroll
+            for (int t = 0; t < 2 * kChunks; ++t)
+              o[n][t][e] *= shrink, o[n][t][e + 2] *= shrink;
+          }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // weights, transposed from (token, column) to (column, token)
+        unsigned p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float p0 = Exp2(score[half][n][2 * r] - top[n][0]), p1 = Exp2(score[half][n][2 * r + 1] - top[n][1]);
+            sum[n][0] += p0, sum[n][1] += p1;
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][r]) : "r"(Pack(p0, p1)));
+          }
+        // V's scales of tokens 2c, 2c + 1 and 2c + 8, 2c + 9 in this lane's group
+        const unsigned char *const values = tile + TileBytes<D>::kCodes + TileBytes<D>::kScales;
+        const unsigned short *const f = reinterpret_cast<const unsigned short *>(values + TileBytes<D>::kCodes) + (16 * half + 2 * c) * kGroups +
+                                        (g >> 1) % kGroups;
+        __half2 scale[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          scale[r] = __halves2half2(__ushort_as_half(f[8 * r * kGroups]), __ushort_as_half(f[(8 * r + 1) * kGroups]));
+#pragma unroll
+        for (int j = 0; j < kChunks; j += 2) {
+          // four 8x8 matrices of 16-bit pieces: tokens 0..7 and 8..15 of chunk j, then of chunk j + 1
+          unsigned v[4];
+          const int token = lane & 15, chunk = j + (lane >> 4);
+          const int swizzled = kChunks == 4 ? chunk ^ ((token >> 1) & 3) : chunk ^ ((token >> 2) & 1);
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(SmemAddress(values + (16 * half + token) * (D / 2) + 16 * swizzled))
+                       : "memory");
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const unsigned u0 = v[2 * k], u1 = v[2 * k + 1], w0 = u0 >> 8, w1 = u1 >> 8;
+            const unsigned a0 = Scaled(Low(u0), 0x64086408u, scale[0]), a1 = Scaled(High(u0), 0x54805480u, scale[0]);
+            const unsigned a2 = Scaled(Low(u1), 0x64086408u, scale[1]), a3 = Scaled(High(u1), 0x54805480u, scale[1]);
+            const unsigned b0 = Scaled(Low(w0), 0x64086408u, scale[0]), b1 = Scaled(High(w0), 0x54805480u, scale[0]);
+            const unsigned b2 = Scaled(Low(w1), 0x64086408u, scale[1]), b3 = Scaled(High(w1), 0x54805480u, scale[1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              MmaF16(o[n][2 * (j + k)], a0, a1, a2, a3, p[n][0], p[n][1]);
+              MmaF16(o[n][2 * (j + k) + 1], b0, b1, b2, b3, p[n][0], p[n][1]);
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    // ---- the warps' maxima, sums and outputs to shared memory (over the rings: every warp is done with its own) ----
+    __syncthreads();
+    if (mine || warp == 0) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = sum[n][e];
+#pragma unroll
+          for (int m = 4; m < 32; m *= 2)
+            x += __shfl_xor_sync(0xffffffffu, x, m);
+          const int column = 8 * n + 2 * c + e;
+          if (g == 0)
+            join_ml[(warp * kColumns + column) * 2] = top[n][e], join_ml[(warp * kColumns + column) * 2 + 1] = x;
+          float *const to = join + (warp * kColumns + column) * kRow;
+#pragma unroll
+          for (int t = 0; t < 2 * kChunks; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) { // chunk t / 2, nibble 2 (t % 2) + r of piece g
+              const int word = 4 * (t / 2) + (g >> 1), dim = 32 * (word % kGroups) + 8 * (word / kGroups) + 4 * (g & 1) + 2 * (t & 1) + r;
+              to[dim] = o[n][t][e + 2 * r];
+            }
+        }
+    }
+    __syncthreads();
+  }
+
+  // Joined over the CTA's warps: maximum, sum and four output values (from `dim`) of a column.
+  static __device__ __forceinline__ float4 Joined(const float *join, const float *join_ml, int warps, int column, int dim, float *top, float *sum) {
+    float m = kNever, l = 0;
+    for (int w = 0; w < warps; ++w)
+      m = fmaxf(m, join_ml[(w * kColumns + column) * 2]);
+    float4 v = make_float4(0, 0, 0, 0);
+    for (int w = 0; w < warps; ++w) {
+      const float f = Exp2(join_ml[(w * kColumns + column) * 2] - m);
+      l += f * join_ml[(w * kColumns + column) * 2 + 1];
+      const float4 x = *reinterpret_cast<const float4 *>(join + (w * kColumns + column) * kRow + dim);
+      v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+    }
+    *top = m, *sum = l;
+    return v;
+  }
+};
+
+// Exclusive prefix sum of one value per thread over the CTA; *total gets the sum.
+__device__ __forceinline__ long long BlockPrefix(long long value, long long *scan, long long *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long inclusive = value;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const long long other = __shfl_up_sync(0xffffffffu, inclusive, d);
+    if (lane >= d)
+      inclusive += other;
+  }
+  if (lane == 31)
+    scan[warp] = inclusive;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    before += w < warp ? scan[w] : 0;
+    all += scan[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + inclusive - value;
+}
+
+template <typename T, int D, int NT> __global__ void __launch_bounds__(kThreads, 1) SplitAttentionKernel(AttentionArgs a) {
+  using P = Piece<T, D, NT>;
+  constexpr int kColumns = P::kColumns;
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ float join_ml[kWarps * kColumns * 2];
+  __shared__ long long scan[kWarps], s_offset;
+  __shared__ int s_sequence, s_last;
+  float *const join = reinterpret_cast<float *>(ring);
+  const int tid = threadIdx.x;
+
+  // ---- this CTA's run of the list: every CTA adds up the same demands ----
+  long long total = 0;
+  for (int s0 = 0; s0 < a.seq.count; s0 += kThreads) {
+    long long part;
+    BlockPrefix(s0 + tid < a.seq.count ? CostOf(a, DemandOf<kColumns>(a, s0 + tid)) : 0, scan, &part);
+    total += part;
+  }
+  // at least one tile for every warp: shorter runs only make more pieces to join
+  const long long share = max(static_cast<long long>(kWarps), (total + gridDim.x - 1) / gridDim.x);
+  const long long begin = blockIdx.x * share, end = min(total, begin + share);
+  if (begin >= end)
+    return;
+  long long before = 0;
+  for (int s0 = 0; s0 < a.seq.count && before <= begin; s0 += kThreads) {
+    long long part;
+    const long long cost = s0 + tid < a.seq.count ? CostOf(a, DemandOf<kColumns>(a, s0 + tid)) : 0, at = before + BlockPrefix(cost, scan, &part);
+    if (begin >= at && begin < at + cost)
+      s_sequence = s0 + tid, s_offset = begin - at;
+    before += part;
+  }
+  __syncthreads();
+  int s = s_sequence;
+  long long offset = s_offset; // tiles into sequence s
+  Demand d = DemandOf<kColumns>(a, s);
+  for (long long at = begin; at < end;) {
+    while (offset >= CostOf(a, d)) { // next sequence with work
+      offset -= CostOf(a, d);
+      d = DemandOf<kColumns>(a, ++s);
+    }
+    const long long unit = offset / d.tiles;
+    const int skip = static_cast<int>(offset - unit * d.tiles), head = static_cast<int>(unit / d.blocks), block = static_cast<int>(unit % d.blocks);
+    const int count = static_cast<int>(min(static_cast<long long>(d.tiles - skip), end - at));
+    P::Run(a, d, s, head, block, d.first + skip, count, ring, join, join_ml);
+    const int warps = min(count, kWarps), columns = min(kColumns, d.rows * a.group - block * kColumns);
+    const bool whole = count == d.tiles;
+    const int slot = at == begin ? 0 : 1;
+    auto partial_of = [&](long long cta, int which) { return a.partial + ((cta * 2 + which) * kColumns) * (D + 2); };
+    auto store = [&](int column, int dim, float4 v, float sum) {
+      const int place = block * kColumns + column, row = place / a.group, h = head * a.group + place % a.group;
+      const float inverse = sum > 0 ? 1.f / sum : 0.f;
+      Store4(static_cast<T *>(a.out) + static_cast<long long>(d.begin + row) * a.out_stride + h * D + dim,
+             make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse));
+    };
+    for (int i = tid; i < columns * (D / 4); i += kThreads) {
+      const int column = i / (D / 4), dim = i % (D / 4) * 4;
+      float top, sum;
+      const float4 v = P::Joined(join, join_ml, warps, column, dim, &top, &sum);
+      if (whole) {
+        store(column, dim, v, sum);
+      } else {
+        float *const to = partial_of(blockIdx.x, slot) + column * (D + 2);
+        *reinterpret_cast<float2 *>(to + dim) = make_float2(v.x, v.y);
+        *reinterpret_cast<float2 *>(to + dim + 2) = make_float2(v.z, v.w);
+        if (dim == 0)
+          *reinterpret_cast<float2 *>(to + D) = make_float2(top, sum);
+      }
+    }
+    if (!whole) {
+      // the unit's pieces lie in the runs of CTAs first .. last
+      const long long unit_begin = at - skip, first = unit_begin / share, last = (unit_begin + d.tiles - 1) / share;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned pieces = static_cast<unsigned>(last - first + 1), arrived = atomicAdd(a.ticket + first, 1u);
+        s_last = arrived == pieces - 1;
+        if (s_last)
+          a.ticket[first] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_last) {
+        const int first_slot = unit_begin == first * share ? 0 : 1;
+        for (int i = tid; i < columns * (D / 4); i += kThreads) {
+          const int column = i / (D / 4), dim = i % (D / 4) * 4;
+          float m = kNever, l = 0;
+          for (long long p = first; p <= last; ++p)
+            m = fmaxf(m, __ldcg(partial_of(p, p == first ? first_slot : 0) + column * (D + 2) + D));
+          float4 v = make_float4(0, 0, 0, 0);
+          for (long long p = first; p <= last; ++p) {
+            const float *const from = partial_of(p, p == first ? first_slot : 0) + column * (D + 2);
+            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + D));
+            const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + dim)), y = __ldcg(reinterpret_cast<const float2 *>(from + dim + 2));
+            const float f = Exp2(ml.x - m);
+            l += f * ml.y;
+            v.x += f * x.x, v.y += f * x.y, v.z += f * y.x, v.w += f * y.y;
+          }
+          store(column, dim, v, l);
+        }
+      }
+    }
+    __syncthreads(); // the rings are free again
+    at += count, offset += count;
+  }
+}
+
+template <typename T, int D, int NT> int LaunchSplit(AttentionArgs a, int sms, cudaStream_t stream) {
+  using P = Piece<T, D, NT>;
+  constexpr size_t kRing = static_cast<size_t>(kWarps) * kStages * TileBytes<D>::kAll, kJoin = sizeof(float) * kWarps * P::kColumns * P::kRow;
+  constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;
+  if (cudaFuncSetAttribute(SplitAttentionKernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess)
+    return PADRA_RESOURCE_EXHAUSTED;
+  SplitAttentionKernel<T, D, NT><<<sms < kMaxGrid ? sms : kMaxGrid, kThreads, kSmem, stream>>>(a);
   return CudaStatus(cudaGetLastError());
 }
 
+// Columns of a block: 16 where a sequence's rows have more than 8 columns.
+template <typename T, int D> int LaunchColumns(const AttentionArgs &a, int sms, cudaStream_t stream) {
+  return static_cast<long long>(a.seq.max_rows) * a.group <= 8 ? LaunchSplit<T, D, 1>(a, sms, stream) : LaunchSplit<T, D, 2>(a, sms, stream);
+}
+
+constexpr size_t kTicketBytes = kMaxGrid * sizeof(unsigned);
+constexpr int kMaxColumns = 16;
+
 } // namespace
 
+size_t AttentionWorkspaceBytes(int head_dim) {
+  if (head_dim != 64 && head_dim != 128)
+    return 0;
+  return kTicketBytes + static_cast<size_t>(kMaxGrid) * 2 * kMaxColumns * (head_dim + 2) * sizeof(float);
+}
+int InitAttentionWorkspace(void *workspace, size_t bytes, cudaStream_t stream) {
+  if (!workspace || bytes < kTicketBytes)
+    return PADRA_INVALID_ARGUMENT;
+  return CudaStatus(cudaMemsetAsync(workspace, 0, kTicketBytes, stream));
+}
+
 int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
-                    long long out_stride, int q_heads, int type, float scale, int window, int *bad, cudaStream_t stream) {
+                    long long out_stride, int q_heads, int type, float scale, int window, void *workspace, size_t workspace_bytes, int *bad,
+                    cudaStream_t stream) {
   KvView c;
   SequenceView s;
-  if (!ViewOf(cache, &c) || !ViewOf(sequences, c, &s) || !bad || q_heads < 1 || q_heads > 4096 || q_heads % c.kv_heads || window < 0)
+  if (!ViewOf(cache, &c) || !ViewOf(sequences, c, &s) || !bad || q_heads < 1 || q_heads > 4096 || q_heads % c.kv_heads || window < 0 ||
+      !std::isfinite(scale))
     return PADRA_INVALID_ARGUMENT;
   if ((c.head_dim != 64 && c.head_dim != 128) || (type != PADRA_ROWS_BF16 && type != PADRA_ROWS_F16))
     return PADRA_UNSUPPORTED;
   if (!RowsOk(q, q_stride, q_heads, c.head_dim) || !RowsOk(out, out_stride, q_heads, c.head_dim))
     return PADRA_INVALID_ARGUMENT;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < AttentionWorkspaceBytes(c.head_dim))
+    return PADRA_INVALID_ARGUMENT;
   if (!s.rows || !s.count)
     return PADRA_OK;
+  int device = 0, sms = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
+    return PADRA_INTERNAL;
+  AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale * 1.4426950408889634f, window,
+                  reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kTicketBytes), static_cast<unsigned *>(workspace), bad};
   if (type == PADRA_ROWS_BF16)
-    return c.head_dim == 64 ? Launch<__nv_bfloat16, 64>(c, s, q, out, q_stride, out_stride, q_heads, scale, window, bad, stream)
-                            : Launch<__nv_bfloat16, 128>(c, s, q, out, q_stride, out_stride, q_heads, scale, window, bad, stream);
-  return c.head_dim == 64 ? Launch<__half, 64>(c, s, q, out, q_stride, out_stride, q_heads, scale, window, bad, stream)
-                          : Launch<__half, 128>(c, s, q, out, q_stride, out_stride, q_heads, scale, window, bad, stream);
+    return c.head_dim == 64 ? LaunchColumns<__nv_bfloat16, 64>(a, sms, stream) : LaunchColumns<__nv_bfloat16, 128>(a, sms, stream);
+  return c.head_dim == 64 ? LaunchColumns<__half, 64>(a, sms, stream) : LaunchColumns<__half, 128>(a, sms, stream);
 }
 
 } // namespace padra

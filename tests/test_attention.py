@@ -48,7 +48,7 @@ def test_cache_and_sequences_are_checked_before_anything_is_enqueued(lib, over, 
     p = 4096
     assert lib.padra_kv_append(C.byref(c), C.byref(s), p, p, 256, 256, None, 1e-6, None, None, None, 0, 0, 0, None, 0, p, None) == want
     assert lib.padra_kv_read(C.byref(c), C.byref(s), p, p, 256, 256, 0, p, None) == want
-    assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None) == want
+    assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, 1 << 40, p, None) == want
 
 
 def test_row_arguments_are_checked(lib):
@@ -56,10 +56,11 @@ def test_row_arguments_are_checked(lib):
 
     c, s, r = structs()
     p = 4096
-    ok = [C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None]
+    ok = [C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, lib.padra_attention_q4_workspace_bytes(64), p, None]
     for at, value, want in [(2, p + 2, B.INVALID_ARGUMENT), (2, None, B.INVALID_ARGUMENT), (3, p + 8, B.INVALID_ARGUMENT), (4, 255, B.INVALID_ARGUMENT),
                             (4, 260, B.INVALID_ARGUMENT), (5, 128, B.INVALID_ARGUMENT), (6, 3, B.INVALID_ARGUMENT), (6, 0, B.INVALID_ARGUMENT),
-                            (7, B.ROWS_F32, B.UNSUPPORTED), (7, 9, B.UNSUPPORTED), (9, -1, B.INVALID_ARGUMENT), (10, None, B.INVALID_ARGUMENT)]:
+                            (7, B.ROWS_F32, B.UNSUPPORTED), (7, 9, B.UNSUPPORTED), (8, math.inf, B.INVALID_ARGUMENT), (9, -1, B.INVALID_ARGUMENT), (10, None, B.INVALID_ARGUMENT),
+                            (10, p + 8, B.INVALID_ARGUMENT), (11, lib.padra_attention_q4_workspace_bytes(64) - 1, B.INVALID_ARGUMENT), (12, None, B.INVALID_ARGUMENT)]:
         args = list(ok)
         args[at] = value
         assert lib.padra_attention_q4(*args) == want, (at, value)
@@ -81,13 +82,22 @@ def test_row_arguments_are_checked(lib):
         assert lib.padra_kv_append(*args) == want, (at, value)
 
 
+def test_attention_workspace(lib):
+    from padra_b200 import binding as B
+
+    assert lib.padra_attention_q4_workspace_bytes(96) == 0
+    assert 0 < lib.padra_attention_q4_workspace_bytes(64) < lib.padra_attention_q4_workspace_bytes(128)
+    assert lib.padra_attention_q4_workspace_init(None, 1 << 20, None) == B.INVALID_ARGUMENT
+    assert lib.padra_attention_q4_workspace_init(4096, 16, None) == B.INVALID_ARGUMENT
+
+
 def test_nothing_to_do_is_not_an_error(lib):
     from padra_b200 import binding as B
 
     p = 4096
     for over in (dict(rows=0), dict(count=0, row_begin=None, context=None)):
         c, s, r = structs(**over)
-        assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, None) == B.OK
+        assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, 0.1, 0, p, 1 << 40, p, None) == B.OK
         assert lib.padra_kv_read(C.byref(c), C.byref(s), p, p, 128, 128, 0, p, None) == B.OK
         assert lib.padra_kv_append(C.byref(c), C.byref(s), p, p, 128, 128, None, 1e-6, None, None, None, 0, 0, 0, None, 0, p, None) == B.OK
     assert lib.padra_qk_norm_rope(p, p, 256, 256, 4, None, None, 0, 0, 0, None, None, 1e-6, p, None, 0, 64, 0, p, None) == B.OK
