@@ -390,12 +390,9 @@ PADRA_API int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *
  * t > p - window.  q, out [rows][q_heads], q_heads a multiple of the cache's kv_heads (heads g * q_heads / kv_heads .. share KV
  * head g); out may not overlap q.  Call after the rows' own K and V have been appended.  A query that is not finite raises
  * *bad and gives zeros.
- * workspace: padra_attention_q4_workspace_bytes(head_dim) bytes (the same for every call), 16-byte aligned, whose tickets have to
- * be zero before the first call (padra_attention_q4_workspace_init, once after allocating it); every call leaves them zero.
- * One workspace serves one stream at a time: calls that share it, captured ones among them, must not overlap on the
- * GPU. */
+ * workspace: padra_attention_q4_workspace_bytes(head_dim) bytes (the same for every call), 16-byte aligned; what it holds before
+ * a call does not matter.  Calls that share it, captured ones among them, must not overlap on the GPU. */
 PADRA_API size_t padra_attention_q4_workspace_bytes(int head_dim);
-PADRA_API int padra_attention_q4_workspace_init(void *workspace, size_t workspace_bytes, padra_stream stream);
 PADRA_API int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out,
                                  long long q_stride, long long out_stride, int q_heads, int type, float scale,
                                  int window, void *workspace, size_t workspace_bytes, int *bad, padra_stream stream);

@@ -155,7 +155,6 @@ class AttentionKernels:
             _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
             n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
             ws = torch.empty(n, dtype=torch.uint8, device=self.bad.device)
-            B.check(self.lib.padra_attention_q4_workspace_init(ws.data_ptr(), n, stream), "padra_attention_q4_workspace_init")
             self._workspace[key] = ws, ws.data_ptr(), n
         return self._workspace[key][1:]
 

@@ -67,7 +67,6 @@ SIGNATURES = {
     "padra_kv_append": ([_p, _p, _p, _p, _l, _l, _p, C.c_double, _p, _p, _p, _l, _l, _i, _p, _i, _p, _p], _i),
     "padra_kv_read": ([_p, _p, _p, _p, _l, _l, _i, _p, _p], _i),
     "padra_attention_q4_workspace_bytes": ([_i], C.c_size_t),
-    "padra_attention_q4_workspace_init": ([_p, C.c_size_t, _p], _i),
     "padra_attention_q4": ([_p, _p, _p, _p, _l, _l, _i, _i, C.c_float, _i, _p, C.c_size_t, _p, _p], _i),
     "padra_codec_ceiling_launch": ([_i, _i, _i, _i, _p, _p], _i),
 }

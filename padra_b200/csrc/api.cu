@@ -338,10 +338,6 @@ size_t padra_attention_q4_workspace_bytes(int head_dim) {
   return AttentionWorkspaceBytes(head_dim);
 }
 
-int padra_attention_q4_workspace_init(void *workspace, size_t workspace_bytes, padra_stream stream) {
-  return InitAttentionWorkspace(workspace, workspace_bytes, S(stream));
-}
-
 int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
                        long long out_stride, int q_heads, int type, float scale, int window, void *workspace, size_t workspace_bytes,
                        int *bad, padra_stream stream) {

@@ -5,8 +5,8 @@
 //   * Work is (sequence, KV head, block of 8 * NT query columns) x 32-token tiles.  All tiles of a call form one list, and
 //     every CTA takes an equal run of it (ends may lie inside a sequence), so neither one long context nor ragged ones
 //     leave SMs idle.  A run's piece of a unit that is not the whole unit leaves maximum, sum and unnormalised output in the
-//     workspace; the CTA that arrives last at such a unit joins the pieces in list order, so results do not depend on
-//     timing.
+//     workspace, and a second kernel, launched as a programmatic dependent, joins the pieces in list order (as the last
+//     CTA's task inside the first kernel that cost fences, tickets, and up to 25 us where one CTA read a hundred pieces).
 //   * A warp owns tiles w, w + 8, ... of the CTA's run, with a private ring of tiles filled by cp.async: no barrier between
 //     warps until the piece ends.
 //   * Scores: K is the MMA's A operand (16 tokens x 16 values), queries the B columns.  A lane's word holds eight codes of one
@@ -28,12 +28,23 @@
 namespace padra {
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
+// Small CTAs, as many to an SM as the registers of a column block leave room for: what a CTA does between two pieces
+// (queries, joining its warps, tickets) runs under the others' tiles.
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+template <int NT> struct Cta {
+  static constexpr int kPerSm = NT == 1 ? 3 : 2;
+};
 constexpr int kTile = 32;   // tokens of a tile
-constexpr int kStages = 5;  // tiles of a warp's ring
-constexpr int kMaxGrid = 1024; // CTAs the workspace provides for
+constexpr int kStages = 4;  // tiles of a warp's ring
+constexpr int kMaxGrid = 512;  // CTAs the workspace provides for
 constexpr float kNever = -1e30f; // the running maximum before any token
 constexpr float kTop = 8.f, kRaise = 15.f; // log2 of the largest weight after a raise / before the next
+
+// The unit that begins in a CTA's run and goes on in others': how many pieces there are (0: no such unit), in which slot this
+// CTA left the first one (the others are in their CTAs' slot 0), and where the output goes.
+struct Split {
+  int pieces, first_slot, row_begin, block, head, columns;
+};
 
 struct AttentionArgs {
   KvView cache;
@@ -42,10 +53,11 @@ struct AttentionArgs {
   void *out;
   long long q_stride, out_stride;
   int q_heads, group; // heads that share a KV head
-  float scale;        // times log2(e)
+  float scale;        // |scale| * log2(e), or 1 where scale is 0
+  float sign;         // of scale: the queries are multiplied by it
   int window;
-  float *partial;     // [grid][2][columns][head_dim + 2]
-  unsigned *ticket;   // [grid]: pieces of the split unit that begins in this CTA's run that have arrived
+  struct Split *split; // [grid]
+  float *partial;      // [grid][2]: outputs [columns][head_dim], then maximum and sum [columns][2]
   int *bad;
 };
 
@@ -79,15 +91,13 @@ __device__ __forceinline__ float Exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void Load8(const __nv_bfloat16 *p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+__device__ __forceinline__ void Widen(uint4 u, const __nv_bfloat16 *, float (&x)[8]) {
   const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
-__device__ __forceinline__ void Load8(const __half *p, float (&x)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4 *>(p);
+__device__ __forceinline__ void Widen(uint4 u, const __half *, float (&x)[8]) {
   const unsigned w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -101,6 +111,11 @@ __device__ __forceinline__ void Store4(__nv_bfloat16 *p, float4 v) {
 }
 __device__ __forceinline__ void Store4(__half *p, float4 v) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(Pack(v.x, v.y), Pack(v.z, v.w));
+}
+
+// a / b of numbers that are nearly always below 2^32, where the division is much cheaper
+__device__ __forceinline__ long long Quotient(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : static_cast<unsigned>(a) / static_cast<unsigned>(b);
 }
 
 // What one sequence asks for: `blocks` column blocks of each KV head, `tiles` tiles for each of them, the first being tile
@@ -134,86 +149,21 @@ template <typename T, int D, int NT> struct Piece {
 
   // column -> row of the sequence and head of the group
   static __device__ __forceinline__ void Run(const AttentionArgs &a, const Demand &d, int s, int head, int block, int first_tile, int count,
-                                             unsigned char *ring, float *join, float *join_ml) {
+                                             unsigned char *ring, float *join, float *join_ml, int2 (*cta_limits)[kColumns]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    int2 *const limits = cta_limits[warp]; // first and last token that a column sees
     const int columns = min(kColumns, d.rows * a.group - block * kColumns);
     const int start = d.context - d.rows; // position of the sequence's first row
 
-    // ---- queries: FP16 after division by a power of two that brings the row's largest value below 2 ----
-    unsigned q[NT][kGroups][4];
-    float factor[NT][2], correction[NT][kGroups][2];
-    int last[NT][2], low[NT][2]; // tokens that columns 2c and 2c + 1 see
-    int least = 0x7fffffff, latest_low = 0;
+    uint4 raw[NT][kGroups]; // on their way while the first tiles are asked for
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int column = 8 * n + g, place = block * kColumns + column, row = place / a.group, h = head * a.group + place % a.group;
-      float x[kGroups][8], most = 0;
-      bool finite = true;
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        if (column < columns && start + row >= 0)
-          Load8(static_cast<const T *>(a.q) + static_cast<long long>(d.begin + row) * a.q_stride + h * D + 32 * i + 8 * c, x[i]);
-        else
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            x[i][j] = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          finite &= isfinite(x[i][j]) != 0;
-          most = fmaxf(most, fabsf(x[i][j]));
-        }
-      }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const bool fine = (__ballot_sync(0xffffffffu, !finite) & (0xfu << (lane & 28))) == 0;
-      if (!fine)
-        Raise(a.bad);
-      const int exponent = most > 0 && fine ? min(126, max(-126, ilogbf(most))) : 0;
-      const float shrink = fine ? ldexpf(1.f, -exponent) : 0.f;
-      float sums[kGroups];
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        float y[8], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          y[j] = fine ? __half2float(__float2half_rn(x[i][j] * shrink)) : 0.f;
-          sum += y[j] * (j & 1 ? -72.f : -1032.f);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          q[n][i][j] = Pack(y[j], y[j + 4]);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sums[i] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
-      }
-      const float mine = a.scale * ldexpf(1.f, exponent);
-      // a row at a negative position sees nothing, nor does one that is not finite, nor a column beyond the last
-      const int to = column < columns && fine ? start + row : -1, from = a.window ? max(0, to - a.window + 1) : 0;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int owner = 4 * (2 * c + e);
-        factor[n][e] = __shfl_sync(0xffffffffu, mine, owner);
-        last[n][e] = __shfl_sync(0xffffffffu, to, owner);
-        low[n][e] = __shfl_sync(0xffffffffu, from, owner);
-#pragma unroll
-        for (int i = 0; i < kGroups; ++i)
-          correction[n][i][e] = __shfl_sync(0xffffffffu, sums[i], owner);
-      }
-      if (column < columns)
-        least = min(least, to), latest_low = max(latest_low, from);
-    }
-#pragma unroll
-    for (int m = 4; m < 32; m *= 2) {
-      least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
-      latest_low = max(latest_low, __shfl_xor_sync(0xffffffffu, latest_low, m));
-    }
-
-    float top[NT][2], sum[NT][2], o[NT][2 * kChunks][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      top[n][0] = top[n][1] = kNever, sum[n][0] = sum[n][1] = 0;
-#pragma unroll
-      for (int t = 0; t < 2 * kChunks; ++t)
-        o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0;
+      for (int i = 0; i < kGroups; ++i)
+        raw[n][i] = column < columns && start + row >= 0
+                        ? *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + static_cast<long long>(d.begin + row) * a.q_stride + h * D + 32 * i + 8 * c)
+                        : make_uint4(0, 0, 0, 0);
     }
 
     // ---- the ring ----
@@ -221,6 +171,14 @@ template <typename T, int D, int NT> struct Piece {
     const int visible_low = a.window ? max(0, start + 1 - a.window) : 0;
     unsigned char *const own_ring = ring + warp * kStages * TileBytes<D>::kAll;
     const unsigned ring_address = SmemAddress(own_ring);
+    // a warp-wide copy takes 512 bytes of codes: 16 per lane, V's swizzled inside the token's row
+    const int code_scale_bytes = a.cache.code_bytes() + a.cache.scale_bytes(), copy_token = lane / kChunks, copy_chunk = lane % kChunks;
+    const unsigned copy_offset = 16 * lane,
+                   swizzled_offset = TileBytes<D>::kCodes + TileBytes<D>::kScales + copy_token * (D / 2) +
+                                     16 * (kChunks == 4 ? copy_chunk ^ ((copy_token >> 1) & 3) : copy_chunk ^ ((copy_token >> 2) & 1));
+    constexpr int kScaleTokens = 256 / D, kScaleLanes = kTile / kScaleTokens; // tokens whose scales fill 16 bytes; lanes for K, as many for V
+    const int scale_of_v = lane / kScaleLanes, scale_from = a.cache.code_bytes() + scale_of_v * code_scale_bytes;
+    const unsigned scale_offset = TileBytes<D>::kCodes + scale_of_v * (TileBytes<D>::kCodes + TileBytes<D>::kScales) + 16 * (lane % kScaleLanes);
     int page_low = -1, page_high = -1; // of this lane's tile among the next 32: first and second 16 tokens
     auto fetch = [&](int i) {
       if (i < mine) {
@@ -240,29 +198,26 @@ template <typename T, int D, int NT> struct Piece {
         }
         const int lo = __shfl_sync(0xffffffffu, page_low, i & 31), hi = __shfl_sync(0xffffffffu, page_high, i & 31);
         const int t0 = (first_tile + warp + i * kWarps) * kTile;
-        const int slot = t0 & (a.cache.page_size - 1), shift_high = a.cache.page_size > 16 ? 0 : 16;
-        // first token of the tile in either page; a half without a page reads page 0's and gets scales of zero
-        const unsigned char *from_low = a.cache.block(max(lo, 0), head), *from_high = a.cache.block(max(hi, 0), head);
-        const unsigned to = ring_address + (i % kStages) * TileBytes<D>::kAll;
-        const int codes = a.cache.code_bytes(), scales = a.cache.scale_bytes();
+        // first token of either half of the tile; a half without a page reads page 0's and gets scales of zero
+        const int slot = t0 & (a.cache.page_size - 1), slot_high = (t0 + 16) & (a.cache.page_size - 1);
+        const unsigned char *const from_low = a.cache.block(max(lo, 0), head), *const from_high = a.cache.block(max(hi, 0), head);
+        const unsigned to = ring_address + (i & (kStages - 1)) * TileBytes<D>::kAll;
         constexpr int kRowsPerCopy = 32 / kChunks, kCopies = kTile / kRowsPerCopy; // tokens per warp-wide copy
-        const int token = lane / kChunks, chunk = lane % kChunks;
-        const int swizzled = kChunks == 4 ? chunk ^ ((token >> 1) & 3) : chunk ^ ((token >> 2) & 1);
 #pragma unroll
-        for (int k = 0; k < kCopies; ++k) {
-          const bool second = k * kRowsPerCopy >= 16;
-          const unsigned char *from = (second ? from_high - shift_high * (D / 2) : from_low) + (slot + k * kRowsPerCopy + token) * (D / 2) + 16 * chunk;
-          const unsigned at = to + (k * kRowsPerCopy + token) * (D / 2);
-          CopyAsync16(at + 16 * chunk, from, 16);
-          CopyAsync16(at + TileBytes<D>::kCodes + TileBytes<D>::kScales + 16 * swizzled, from + codes + scales, 16);
+        for (int h = 0; h < 2; ++h) {
+          const unsigned char *const from = (h ? from_high + slot_high * (D / 2) : from_low + slot * (D / 2)) + 16 * lane;
+          const unsigned char *const from_v = from + code_scale_bytes;
+#pragma unroll
+          for (int k = h * kCopies / 2; k < (h + 1) * kCopies / 2; ++k) {
+            CopyAsync16(to + copy_offset + k * 512, from + (k - h * kCopies / 2) * 512, 16);
+            CopyAsync16(to + swizzled_offset + k * 512, from_v + (k - h * kCopies / 2) * 512, 16);
+          }
         }
-        constexpr int kTokens = 256 / D, kLanes = kTile / kTokens; // tokens whose scales fit 16 bytes; lanes for K, as many for V
-        if (lane < 2 * kLanes) {
-          const int which = lane / kLanes, t = lane % kLanes * kTokens;
-          const bool second = t >= 16;
-          const int valid = (second ? hi : lo) < 0 ? 0 : max(0, min(kTokens, d.context - t0 - t));
-          const unsigned char *from = (second ? from_high - shift_high * (D / 16) : from_low) + codes + which * (codes + scales) + (slot + t) * (D / 16);
-          CopyAsync16(to + TileBytes<D>::kCodes + which * (TileBytes<D>::kCodes + TileBytes<D>::kScales) + t * (D / 16), from, valid * (D / 16));
+        if (lane < 2 * kScaleLanes) {
+          const int t = lane % kScaleLanes * kScaleTokens;
+          const int valid = (t >= 16 ? hi : lo) < 0 ? 0 : max(0, min(kScaleTokens, d.context - t0 - t));
+          const unsigned char *const from = t >= 16 ? from_high + (slot_high + t - 16) * (D / 16) : from_low + (slot + t) * (D / 16);
+          CopyAsync16(to + scale_offset, from + scale_from, valid * (D / 16));
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -271,11 +226,84 @@ template <typename T, int D, int NT> struct Piece {
     for (int i = 0; i < kStages - 1; ++i)
       fetch(i);
 
+    // ---- queries: FP16 after division by a power of two that brings the row's largest value below 2 ----
+    unsigned q[NT][kGroups][4];
+    float factor[NT][2], correction[NT][kGroups][2];
+    int least = 0x7fffffff, latest_low = 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int column = 8 * n + g, place = block * kColumns + column, row = place / a.group;
+      float x[kGroups][8], most = 0;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        Widen(raw[n][i], static_cast<const T *>(nullptr), x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          finite &= isfinite(x[i][j]) != 0;
+          most = fmaxf(most, fabsf(x[i][j]));
+        }
+      }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const bool fine = (__ballot_sync(0xffffffffu, !finite) & (0xfu << (lane & 28))) == 0;
+      if (!fine)
+        Raise(a.bad);
+      const int exponent = most > 0 && fine ? min(126, max(-126, ilogbf(most))) : 0;
+      const float shrink = fine ? ldexpf(1.f, -exponent) : 0.f;
+      float sums[kGroups];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        float y[8], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          y[j] = fine ? __half2float(__float2half_rn(x[i][j] * shrink)) * a.sign : 0.f;
+          sum += y[j] * (j & 1 ? -72.f : -1032.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          q[n][i][j] = Pack(y[j], y[j + 4]);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sums[i] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+      }
+      const float mine = a.scale * ldexpf(1.f, exponent);
+      // a row at a negative position sees nothing, nor does one that is not finite, nor a column beyond the last
+      const int to = column < columns && fine ? start + row : -1, from = a.window ? max(0, to - a.window + 1) : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int owner = 4 * (2 * c + e);
+        factor[n][e] = __shfl_sync(0xffffffffu, mine, owner);
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i)
+          correction[n][i][e] = __shfl_sync(0xffffffffu, sums[i], owner);
+      }
+      if (column < columns)
+        least = min(least, to), latest_low = max(latest_low, from);
+      if (c == 0)
+        limits[column] = make_int2(from, to);
+    }
+#pragma unroll
+    for (int m = 4; m < 32; m *= 2) {
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, m));
+      latest_low = max(latest_low, __shfl_xor_sync(0xffffffffu, latest_low, m));
+    }
+
+    __syncwarp();
+
+    float top[NT][2], sum[NT][2], o[NT][2 * kChunks][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      top[n][0] = top[n][1] = kNever, sum[n][0] = sum[n][1] = 0;
+#pragma unroll
+      for (int t = 0; t < 2 * kChunks; ++t)
+        o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0;
+    }
+
     for (int i = 0; i < mine; ++i) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp(); // the tile is here for every lane, and nobody reads the slot that is filled next
       fetch(i + kStages - 1);
-      const unsigned char *const tile = own_ring + (i % kStages) * TileBytes<D>::kAll;
+      const unsigned char *const tile = own_ring + (i & (kStages - 1)) * TileBytes<D>::kAll;
       const int t0 = (first_tile + warp + i * kWarps) * kTile;
       const bool edge = t0 + kTile - 1 > least || t0 < latest_low;
 
@@ -316,32 +344,37 @@ template <typename T, int D, int NT> struct Piece {
           }
         }
       }
-      // scores in units of log2, masked
-      float most = kNever;
+      if (edge) { // tokens that some column does not see
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = score[half][n][e] * factor[n][e & 1];
-            if (edge) {
+            for (int e = 0; e < 4; ++e) {
               const int t = t0 + 16 * half + 8 * (e >> 1) + g;
-              x = t > last[n][e & 1] || t < low[n][e & 1] ? -INFINITY : x;
+              const int2 seen = limits[8 * n + 2 * c + (e & 1)];
+              if (t < seen.x || t > seen.y)
+                score[half][n][e] = -INFINITY;
             }
-            score[half][n][e] = x;
-            most = fmaxf(most, x - top[n][e & 1]);
-          }
-      if (__any_sync(0xffffffffu, most > kRaise)) {
+      }
+      float most[NT][2], over = kNever; // largest score of a column, and by how much log2 of a weight is largest
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          most[n][e] = fmaxf(fmaxf(score[0][n][e], score[0][n][e + 2]), fmaxf(score[1][n][e], score[1][n][e + 2]));
+          over = fmaxf(over, fmaf(most[n][e], factor[n][e], -top[n][e]));
+        }
+      if (__any_sync(0xffffffffu, over > kRaise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(fmaxf(score[0][n][e], score[0][n][e + 2]), fmaxf(score[1][n][e], score[1][n][e + 2]));
+            float x = most[n][e];
 #pragma unroll
             for (int m = 4; m < 32; m *= 2)
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
-            const float next = fmaxf(top[n][e], x - kTop), shrink = Exp2(top[n][e] - next);
+            const float next = fmaxf(top[n][e], fmaf(x, factor[n][e], -kTop)), shrink = Exp2(top[n][e] - next);
             top[n][e] = next, sum[n][e] *= shrink;
 #pragma unroll
             for (int t = 0; t < 2 * kChunks; ++t)
@@ -356,7 +389,8 @@ template <typename T, int D, int NT> struct Piece {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float p0 = Exp2(score[half][n][2 * r] - top[n][0]), p1 = Exp2(score[half][n][2 * r + 1] - top[n][1]);
+            const float p0 = Exp2(fmaf(score[half][n][2 * r], factor[n][0], -top[n][0])),
+                        p1 = Exp2(fmaf(score[half][n][2 * r + 1], factor[n][1], -top[n][1]));
             sum[n][0] += p0, sum[n][1] += p1;
             asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][r]) : "r"(Pack(p0, p1)));
           }
@@ -423,19 +457,35 @@ template <typename T, int D, int NT> struct Piece {
     __syncthreads();
   }
 
-  // Joined over the CTA's warps: maximum, sum and four output values (from `dim`) of a column.
-  static __device__ __forceinline__ float4 Joined(const float *join, const float *join_ml, int warps, int column, int dim, float *top, float *sum) {
-    float m = kNever, l = 0;
-    for (int w = 0; w < warps; ++w)
-      m = fmaxf(m, join_ml[(w * kColumns + column) * 2]);
-    float4 v = make_float4(0, 0, 0, 0);
-    for (int w = 0; w < warps; ++w) {
-      const float f = Exp2(join_ml[(w * kColumns + column) * 2] - m);
-      l += f * join_ml[(w * kColumns + column) * 2 + 1];
-      const float4 x = *reinterpret_cast<const float4 *>(join + (w * kColumns + column) * kRow + dim);
-      v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+  // Joins the CTA's warps: join_ml becomes the weight of every (warp, column), ml the column's maximum and sum.
+  static __device__ __forceinline__ void Weigh(float *join_ml, float2 *ml, int warps, int columns) {
+    const int column = threadIdx.x;
+    if (column < columns) {
+      float m = kNever, l = 0, f[kWarps];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        m = fmaxf(m, w < warps ? join_ml[(w * kColumns + column) * 2] : kNever);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        f[w] = w < warps ? Exp2(join_ml[(w * kColumns + column) * 2] - m) : 0.f;
+        l += w < warps ? f[w] * join_ml[(w * kColumns + column) * 2 + 1] : 0.f;
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        join_ml[(w * kColumns + column) * 2] = f[w];
+      ml[column] = make_float2(m, l);
     }
-    *top = m, *sum = l;
+    __syncthreads();
+  }
+  static __device__ __forceinline__ float4 Joined(const float *join, const float *join_ml, int warps, int column, int dim) {
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      if (w < warps) {
+        const float f = join_ml[(w * kColumns + column) * 2];
+        const float4 x = *reinterpret_cast<const float4 *>(join + (w * kColumns + column) * kRow + dim);
+        v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
+      }
     return v;
   }
 };
@@ -464,108 +514,155 @@ __device__ __forceinline__ long long BlockPrefix(long long value, long long *sca
   return before + inclusive - value;
 }
 
-template <typename T, int D, int NT> __global__ void __launch_bounds__(kThreads, 1) SplitAttentionKernel(AttentionArgs a) {
+// Where a CTA leaves a piece of a unit: which = 0 for the first unit of its run, 1 for the last.
+template <int D, int Columns> __device__ __forceinline__ float *PartialOf(const AttentionArgs &a, long long cta, int which) {
+  return a.partial + (cta * 2 + which) * (Columns * (D + 2));
+}
+template <typename T, int D, int Columns>
+__device__ __forceinline__ void StoreOutput(const AttentionArgs &a, int row_begin, int block, int head, int column, int dim, float4 v, float sum) {
+  const int place = block * Columns + column, row = place / a.group, h = head * a.group + place % a.group;
+  const float inverse = sum > 0 ? 1.f / sum : 0.f;
+  Store4(static_cast<T *>(a.out) + static_cast<long long>(row_begin + row) * a.out_stride + h * D + dim,
+         make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse));
+}
+
+template <typename T, int D, int NT> __global__ void __launch_bounds__(kThreads, Cta<NT>::kPerSm) SplitAttentionKernel(const __grid_constant__ AttentionArgs a) {
   using P = Piece<T, D, NT>;
   constexpr int kColumns = P::kColumns;
   extern __shared__ __align__(128) unsigned char ring[];
   __shared__ float join_ml[kWarps * kColumns * 2];
+  __shared__ int2 limits[kWarps][kColumns];
   __shared__ long long scan[kWarps], s_offset;
-  __shared__ int s_sequence, s_last;
+  __shared__ float2 s_ml[kColumns];
+  __shared__ Demand s_demand;
+  __shared__ int s_sequence;
   float *const join = reinterpret_cast<float *>(ring);
   const int tid = threadIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); // the joining kernel fills SMs as CTAs leave
 
-  // ---- this CTA's run of the list: every CTA adds up the same demands ----
-  long long total = 0;
+  // ---- this CTA's run of the list: every CTA adds up the same demands, one sequence per thread at a time ----
+  Demand mine{};
+  long long total = 0, at_mine = 0, cost_mine = 0;
   for (int s0 = 0; s0 < a.seq.count; s0 += kThreads) {
     long long part;
-    BlockPrefix(s0 + tid < a.seq.count ? CostOf(a, DemandOf<kColumns>(a, s0 + tid)) : 0, scan, &part);
+    mine = s0 + tid < a.seq.count ? DemandOf<kColumns>(a, s0 + tid) : Demand{};
+    cost_mine = CostOf(a, mine);
+    at_mine = total + BlockPrefix(cost_mine, scan, &part);
     total += part;
   }
   // at least one tile for every warp: shorter runs only make more pieces to join
-  const long long share = max(static_cast<long long>(kWarps), (total + gridDim.x - 1) / gridDim.x);
+  const long long share = max(static_cast<long long>(kWarps), Quotient(total + gridDim.x - 1, gridDim.x));
   const long long begin = blockIdx.x * share, end = min(total, begin + share);
+  if (tid == 0)
+    a.split[blockIdx.x].pieces = 0;
   if (begin >= end)
     return;
-  long long before = 0;
-  for (int s0 = 0; s0 < a.seq.count && before <= begin; s0 += kThreads) {
-    long long part;
-    const long long cost = s0 + tid < a.seq.count ? CostOf(a, DemandOf<kColumns>(a, s0 + tid)) : 0, at = before + BlockPrefix(cost, scan, &part);
-    if (begin >= at && begin < at + cost)
-      s_sequence = s0 + tid, s_offset = begin - at;
-    before += part;
+  if (a.seq.count <= kThreads) { // the demands are still in the threads' registers
+    if (begin >= at_mine && begin < at_mine + cost_mine)
+      s_sequence = tid, s_offset = begin - at_mine, s_demand = mine;
+  } else {
+    long long before = 0;
+    for (int s0 = 0; s0 < a.seq.count && before <= begin; s0 += kThreads) {
+      long long part;
+      mine = s0 + tid < a.seq.count ? DemandOf<kColumns>(a, s0 + tid) : Demand{};
+      cost_mine = CostOf(a, mine);
+      at_mine = before + BlockPrefix(cost_mine, scan, &part);
+      if (begin >= at_mine && begin < at_mine + cost_mine)
+        s_sequence = s0 + tid, s_offset = begin - at_mine, s_demand = mine;
+      before += part;
+    }
   }
   __syncthreads();
   int s = s_sequence;
   long long offset = s_offset; // tiles into sequence s
-  Demand d = DemandOf<kColumns>(a, s);
+  Demand d = s_demand;
   for (long long at = begin; at < end;) {
     while (offset >= CostOf(a, d)) { // next sequence with work
       offset -= CostOf(a, d);
       d = DemandOf<kColumns>(a, ++s);
     }
-    const long long unit = offset / d.tiles;
-    const int skip = static_cast<int>(offset - unit * d.tiles), head = static_cast<int>(unit / d.blocks), block = static_cast<int>(unit % d.blocks);
+    const long long unit = Quotient(offset, d.tiles);
+    const int skip = static_cast<int>(offset - unit * d.tiles), head = static_cast<int>(Quotient(unit, d.blocks)), block = static_cast<int>(unit - static_cast<long long>(head) * d.blocks);
     const int count = static_cast<int>(min(static_cast<long long>(d.tiles - skip), end - at));
-    P::Run(a, d, s, head, block, d.first + skip, count, ring, join, join_ml);
+    P::Run(a, d, s, head, block, d.first + skip, count, ring, join, join_ml, limits);
     const int warps = min(count, kWarps), columns = min(kColumns, d.rows * a.group - block * kColumns);
+    P::Weigh(join_ml, s_ml, warps, columns);
     const bool whole = count == d.tiles;
     const int slot = at == begin ? 0 : 1;
-    auto partial_of = [&](long long cta, int which) { return a.partial + ((cta * 2 + which) * kColumns) * (D + 2); };
-    auto store = [&](int column, int dim, float4 v, float sum) {
-      const int place = block * kColumns + column, row = place / a.group, h = head * a.group + place % a.group;
-      const float inverse = sum > 0 ? 1.f / sum : 0.f;
-      Store4(static_cast<T *>(a.out) + static_cast<long long>(d.begin + row) * a.out_stride + h * D + dim,
-             make_float4(v.x * inverse, v.y * inverse, v.z * inverse, v.w * inverse));
-    };
     for (int i = tid; i < columns * (D / 4); i += kThreads) {
       const int column = i / (D / 4), dim = i % (D / 4) * 4;
-      float top, sum;
-      const float4 v = P::Joined(join, join_ml, warps, column, dim, &top, &sum);
+      const float4 v = P::Joined(join, join_ml, warps, column, dim);
       if (whole) {
-        store(column, dim, v, sum);
+        StoreOutput<T, D, kColumns>(a, d.begin, block, head, column, dim, v, s_ml[column].y);
       } else {
-        float *const to = partial_of(blockIdx.x, slot) + column * (D + 2);
-        *reinterpret_cast<float2 *>(to + dim) = make_float2(v.x, v.y);
-        *reinterpret_cast<float2 *>(to + dim + 2) = make_float2(v.z, v.w);
+        float *const to = PartialOf<D, kColumns>(a, blockIdx.x, slot);
+        *reinterpret_cast<float4 *>(to + column * D + dim) = v;
         if (dim == 0)
-          *reinterpret_cast<float2 *>(to + D) = make_float2(top, sum);
+          *reinterpret_cast<float2 *>(to + kColumns * D + 2 * column) = s_ml[column];
       }
     }
-    if (!whole) {
-      // the unit's pieces lie in the runs of CTAs first .. last
-      const long long unit_begin = at - skip, first = unit_begin / share, last = (unit_begin + d.tiles - 1) / share;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        const unsigned pieces = static_cast<unsigned>(last - first + 1), arrived = atomicAdd(a.ticket + first, 1u);
-        s_last = arrived == pieces - 1;
-        if (s_last)
-          a.ticket[first] = 0;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        const int first_slot = unit_begin == first * share ? 0 : 1;
-        for (int i = tid; i < columns * (D / 4); i += kThreads) {
-          const int column = i / (D / 4), dim = i % (D / 4) * 4;
-          float m = kNever, l = 0;
-          for (long long p = first; p <= last; ++p)
-            m = fmaxf(m, __ldcg(partial_of(p, p == first ? first_slot : 0) + column * (D + 2) + D));
-          float4 v = make_float4(0, 0, 0, 0);
-          for (long long p = first; p <= last; ++p) {
-            const float *const from = partial_of(p, p == first ? first_slot : 0) + column * (D + 2);
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + D));
-            const float2 x = __ldcg(reinterpret_cast<const float2 *>(from + dim)), y = __ldcg(reinterpret_cast<const float2 *>(from + dim + 2));
-            const float f = Exp2(ml.x - m);
-            l += f * ml.y;
-            v.x += f * x.x, v.y += f * x.y, v.z += f * y.x, v.w += f * y.y;
-          }
-          store(column, dim, v, l);
-        }
-      }
+    if (!whole && !skip && tid == 0) { // only the last unit of a run can go on in the next
+      const long long last = Quotient(at + d.tiles - 1, share);
+      a.split[blockIdx.x] = Split{static_cast<int>(last - blockIdx.x) + 1, slot, d.begin, block, head, columns};
     }
     __syncthreads(); // the rings are free again
     at += count, offset += count;
+  }
+}
+
+// Joins the pieces of the unit that begins in run blockIdx.x, columns y, y + gridDim.y, ...: kJoinWarps warps read a column's pieces.
+constexpr int kJoinWarps = 8;
+template <typename T, int D, int Columns> __global__ void __launch_bounds__(kJoinWarps * 32) JoinKernel(const __grid_constant__ AttentionArgs a) {
+  constexpr int kLanes = D / 4, kSide = 32 / kLanes, kAtOnce = kJoinWarps * kSide; // pieces that the CTA reads at a time
+  __shared__ float s_sides[kAtOnce];
+  __shared__ float4 s_out[kAtOnce][kLanes];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Split split = a.split[blockIdx.x];
+  const int lane = threadIdx.x & 31, side = threadIdx.x / kLanes, dim = threadIdx.x % kLanes * 4;
+  for (int column = blockIdx.y; column < (split.pieces ? split.columns : 0); column += gridDim.y) {
+    auto piece = [&](int p) { return PartialOf<D, Columns>(a, blockIdx.x + p, p ? 0 : split.first_slot); };
+    // every warp goes over the maxima of all pieces (they are few and in L2)
+    float top = kNever, sum = 0;
+    for (int p = lane; p < split.pieces; p += 32)
+      top = fmaxf(top, __ldcg(piece(p) + Columns * D + 2 * column));
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2)
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    float4 v = make_float4(0, 0, 0, 0);
+    constexpr int kFlight = 4;
+    for (int p0 = side; p0 < split.pieces; p0 += kAtOnce * kFlight) {
+      float4 x[kFlight];
+      float2 ml[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j)
+        if (p0 + j * kAtOnce < split.pieces) {
+          const float *const from = piece(p0 + j * kAtOnce);
+          x[j] = __ldcg(reinterpret_cast<const float4 *>(from + column * D + dim));
+          ml[j] = __ldcg(reinterpret_cast<const float2 *>(from + Columns * D + 2 * column));
+        }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j)
+        if (p0 + j * kAtOnce < split.pieces) {
+          const float f = Exp2(ml[j].x - top);
+          sum += f * ml[j].y;
+          v.x += f * x[j].x, v.y += f * x[j].y, v.z += f * x[j].z, v.w += f * x[j].w;
+        }
+    }
+    s_out[side][dim / 4] = v;
+    if (dim == 0)
+      s_sides[side] = sum;
+    __syncthreads();
+    if (threadIdx.x < kLanes) {
+      for (int i = 1; i < kAtOnce; ++i) {
+        const float4 x = s_out[i][threadIdx.x];
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      sum = 0;
+      for (int i = 0; i < kAtOnce; ++i)
+        sum += s_sides[i];
+      StoreOutput<T, D, Columns>(a, split.row_begin, split.block, split.head, column, dim, v, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -575,8 +672,17 @@ template <typename T, int D, int NT> int LaunchSplit(AttentionArgs a, int sms, c
   constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;
   if (cudaFuncSetAttribute(SplitAttentionKernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem)) != cudaSuccess)
     return PADRA_RESOURCE_EXHAUSTED;
-  SplitAttentionKernel<T, D, NT><<<sms < kMaxGrid ? sms : kMaxGrid, kThreads, kSmem, stream>>>(a);
-  return CudaStatus(cudaGetLastError());
+  const int grid = min(sms * Cta<NT>::kPerSm, kMaxGrid);
+  SplitAttentionKernel<T, D, NT><<<grid, kThreads, kSmem, stream>>>(a);
+  if (cudaGetLastError() != cudaSuccess)
+    return PADRA_INTERNAL;
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.gridDim = dim3(grid, 4), config.blockDim = dim3(kJoinWarps * 32), config.stream = stream;
+  config.attrs = &attribute, config.numAttrs = 1;
+  return CudaStatus(cudaLaunchKernelEx(&config, JoinKernel<T, D, P::kColumns>, a));
 }
 
 // Columns of a block: 16 where a sequence's rows have more than 8 columns.
@@ -584,7 +690,8 @@ template <typename T, int D> int LaunchColumns(const AttentionArgs &a, int sms, 
   return static_cast<long long>(a.seq.max_rows) * a.group <= 8 ? LaunchSplit<T, D, 1>(a, sms, stream) : LaunchSplit<T, D, 2>(a, sms, stream);
 }
 
-constexpr size_t kTicketBytes = kMaxGrid * sizeof(unsigned);
+constexpr size_t kSplitBytes = kMaxGrid * sizeof(Split);
+static_assert(kSplitBytes % 16 == 0, "the pieces behind are read 16 bytes at a time");
 constexpr int kMaxColumns = 16;
 
 } // namespace
@@ -592,14 +699,8 @@ constexpr int kMaxColumns = 16;
 size_t AttentionWorkspaceBytes(int head_dim) {
   if (head_dim != 64 && head_dim != 128)
     return 0;
-  return kTicketBytes + static_cast<size_t>(kMaxGrid) * 2 * kMaxColumns * (head_dim + 2) * sizeof(float);
+  return kSplitBytes + static_cast<size_t>(kMaxGrid) * 2 * kMaxColumns * (head_dim + 2) * sizeof(float);
 }
-int InitAttentionWorkspace(void *workspace, size_t bytes, cudaStream_t stream) {
-  if (!workspace || bytes < kTicketBytes)
-    return PADRA_INVALID_ARGUMENT;
-  return CudaStatus(cudaMemsetAsync(workspace, 0, kTicketBytes, stream));
-}
-
 int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
                     long long out_stride, int q_heads, int type, float scale, int window, void *workspace, size_t workspace_bytes, int *bad,
                     cudaStream_t stream) {
@@ -619,8 +720,9 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
     return PADRA_INTERNAL;
-  AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale * 1.4426950408889634f, window,
-                  reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kTicketBytes), static_cast<unsigned *>(workspace), bad};
+  AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * 1.4426950408889634f : 1.f,
+                  scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f, window,
+                  static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), bad};
   if (type == PADRA_ROWS_BF16)
     return c.head_dim == 64 ? LaunchColumns<__nv_bfloat16, 64>(a, sms, stream) : LaunchColumns<__nv_bfloat16, 128>(a, sms, stream);
   return c.head_dim == 64 ? LaunchColumns<__half, 64>(a, sms, stream) : LaunchColumns<__half, 128>(a, sms, stream);

@@ -97,7 +97,6 @@ int LaunchKvAppend(const padra_kv_cache *cache, const padra_sequences *sequences
 int LaunchKvRead(const padra_kv_cache *cache, const padra_sequences *sequences, void *k_out, void *v_out, long long k_stride, long long v_stride,
                  int type, int *bad, cudaStream_t stream);
 size_t AttentionWorkspaceBytes(int head_dim);
-int InitAttentionWorkspace(void *workspace, size_t bytes, cudaStream_t stream);
 int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out, long long q_stride,
                     long long out_stride, int q_heads, int type, float scale, int window, void *workspace, size_t workspace_bytes, int *bad,
                     cudaStream_t stream);
