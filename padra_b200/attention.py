@@ -75,13 +75,25 @@ class Rotary:
         self.ref = C.addressof(self.struct)
 
 
-def _heads(x: torch.Tensor, what: str) -> int:
-    """Row stride of a [rows][heads][head_dim] tensor whose heads lie side by side."""
-    heads, dim = x.shape[1:]
+def _row_stride(x: torch.Tensor, rows: int, dim: int, dtype: torch.dtype, what: str) -> int:
+    """Checks a [rows][heads][dim] row array, whose heads lie side by side, and returns its stride per row."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim or x.dtype is not dtype:
+        raise ValueError(f"{what}: want [{rows}][heads][{dim}] of {dtype}, got {list(shape)} of {x.dtype}")
+    if x.is_contiguous():
+        return shape[1] * dim
     stride = x.stride()
-    if stride[2] != 1 or (heads > 1 and stride[1] != dim):
-        raise ValueError(f"{what}: heads of a row lie side by side")
-    return stride[0] if x.shape[0] > 1 else heads * dim
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != dim):
+        raise ValueError(f"{what}: the heads of a row lie side by side")
+    return stride[0]
+
+
+def _weight(w: torch.Tensor | None, dim: int) -> int | None:
+    if w is None:
+        return None
+    if (w.dtype is not torch.bfloat16 and w.dtype is not torch.uint16) or w.numel() != dim or not w.is_contiguous():
+        raise ValueError("norm weights are BF16 vectors of head_dim values")
+    return w.data_ptr()
 
 
 class AttentionKernels:
@@ -90,7 +102,7 @@ class AttentionKernels:
     def __init__(self, device="cuda"):
         self.lib = B.load()
         self.bad = torch.zeros(1, dtype=torch.int32, device=device)
-        self._bad = self.bad.data_ptr()
+        self._bad, self._device = self.bad.data_ptr(), self.bad.get_device()
         self._workspace = {}  # (stream, head_dim) -> workspace: calls on one stream follow one another
 
     def reset_bad(self):
@@ -99,71 +111,95 @@ class AttentionKernels:
     def bad_flag(self) -> int:
         return int(self.bad.item())
 
-    @staticmethod
-    def _weight(w, dim):
-        if w is None:
-            return None
-        _need(w.dtype in (torch.bfloat16, torch.uint16) and w.numel() == dim and w.is_contiguous(), "norm weights are BF16 vectors of head_dim values")
-        return w.data_ptr()
+    def _stream(self, stream) -> int:
+        # the library launches on the current device
+        if torch._C._cuda_getDevice() != self._device:
+            raise ValueError(f"the current device is not cuda:{self._device}, which these kernels were made for")
+        return torch._C._cuda_getCurrentRawStream(self._device) if stream is None else stream.cuda_stream
 
     def qk_norm_rope(self, q, k, positions, rotary=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None, stream=None):
         """Per-head RMS norm (where a weight is given) and rotation of q and k (k may be None); returns (q_out, k_out)."""
         rows, q_heads, dim = q.shape
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
-        _need(q_out.shape == q.shape and q_out.dtype == q.dtype, "q_out is shaped and typed as q")
-        _need(positions is None or (positions.dtype == torch.int32 and positions.numel() == rows and positions.is_contiguous()), "positions: int32 [rows]")
-        k_args = (None, None, 0, 0, 0)
+        dtype = q.dtype
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
+        if positions is not None:
+            _need(positions.dtype is torch.int32 and positions.numel() == rows and positions.is_contiguous(), "positions: int32 [rows]")
         if k is not None:
-            k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
-            _need(k.shape[::2] == (rows, dim) and k.dtype == q.dtype and k_out.shape == k.shape and k_out.dtype == k.dtype, "k and k_out: rows, head size and type of q")
-            k_args = (k.data_ptr(), k_out.data_ptr(), _heads(k, "k"), _heads(k_out, "k_out"), k.shape[1])
-        B.check(self.lib.padra_qk_norm_rope(q.data_ptr(), q_out.data_ptr(), _heads(q, "q"), _heads(q_out, "q_out"), q_heads, *k_args,
-                                            self._weight(q_weight, dim), self._weight(k_weight, dim), eps, B.ptr(positions),
-                                            rotary and rotary.ref, rows, dim, ROWS_TYPE[q.dtype], self._bad, B.stream_handle(stream)),
-                "padra_qk_norm_rope")
+            if k_out is None:
+                k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            k_heads = k.shape[1]
+            _need(k_out.shape[1] == k_heads, "k_out has as many heads as k")
+            k_args = (k.data_ptr(), k_out.data_ptr(), _row_stride(k, rows, dim, dtype, "k"), _row_stride(k_out, rows, dim, dtype, "k_out"), k_heads)
+        else:
+            k_args = (None, None, 0, 0, 0)
+        status = self.lib.padra_qk_norm_rope(
+            q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(q_out, rows, dim, dtype, "q_out"), q_heads, *k_args,
+            _weight(q_weight, dim), _weight(k_weight, dim), eps, None if positions is None else positions.data_ptr(), rotary and rotary.ref, rows, dim,
+            ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
+        if status:
+            raise B.PadraError(status, "padra_qk_norm_rope")
         return q_out, k_out
 
     def append(self, cache, sequences, k, v, rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None, q_out=None, stream=None):
         """Appends the rows' K (normed, rotated) and V; with q also norms and rotates the rows' queries and returns them."""
-        dim, shape = cache.head_dim, (sequences.rows, cache.kv_heads, cache.head_dim)
-        _need(k.shape == shape and v.shape == shape and v.dtype == k.dtype, "k and v are [rows][kv_heads][head_dim] of one type")
-        q_args = (None, None, 0, 0, 0, None)
+        rows, dim, dtype = sequences.rows, cache.head_dim, k.dtype
+        _need(k.shape[1] == cache.kv_heads and v.shape[1] == cache.kv_heads, "k and v have the cache's heads")
         if q is not None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
-            _need(q.shape[::2] == shape[::2] and q.dtype == k.dtype and q_out.shape == q.shape and q_out.dtype == q.dtype, "q and q_out: rows, head size and type of k")
-            q_args = (q.data_ptr(), q_out.data_ptr(), _heads(q, "q"), _heads(q_out, "q_out"), q.shape[1], self._weight(q_weight, dim))
-        B.check(self.lib.padra_kv_append(cache.ref, sequences.ref, k.data_ptr(), v.data_ptr(), _heads(k, "k"), _heads(v, "v"),
-                                         self._weight(k_weight, dim), eps, rotary and rotary.ref, *q_args, ROWS_TYPE[k.dtype], self._bad,
-                                         B.stream_handle(stream)), "padra_kv_append")
+            if q_out is None:
+                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            q_heads = q.shape[1]
+            _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
+            q_args = (q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(q_out, rows, dim, dtype, "q_out"), q_heads,
+                      _weight(q_weight, dim))
+        else:
+            q_args = (None, None, 0, 0, 0, None)
+        status = self.lib.padra_kv_append(
+            cache.ref, sequences.ref, k.data_ptr(), v.data_ptr(), _row_stride(k, rows, dim, dtype, "k"), _row_stride(v, rows, dim, dtype, "v"),
+            _weight(k_weight, dim), eps, rotary and rotary.ref, *q_args, ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
+        if status:
+            raise B.PadraError(status, "padra_kv_append")
         return q_out
 
     def read(self, cache, sequences, k_out=None, v_out=None, dtype=torch.bfloat16, stream=None):
         """The values of the cached tokens at the rows' positions; returns (k_out, v_out)."""
-        shape = (sequences.rows, cache.kv_heads, cache.head_dim)
-        k_out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if k_out is None else k_out
-        v_out = torch.empty(shape, dtype=dtype, device=cache.pool.device) if v_out is None else v_out
-        _need(k_out.shape == shape and v_out.shape == shape and v_out.dtype == k_out.dtype, "k_out and v_out are [rows][kv_heads][head_dim] of one type")
-        B.check(self.lib.padra_kv_read(cache.ref, sequences.ref, k_out.data_ptr(), v_out.data_ptr(), _heads(k_out, "k_out"), _heads(v_out, "v_out"),
-                                       ROWS_TYPE[k_out.dtype], self._bad, B.stream_handle(stream)), "padra_kv_read")
+        rows, heads, dim = sequences.rows, cache.kv_heads, cache.head_dim
+        if k_out is None:
+            k_out = torch.empty((rows, heads, dim), dtype=dtype, device=cache.pool.device)
+        if v_out is None:
+            v_out = torch.empty((rows, heads, dim), dtype=k_out.dtype, device=cache.pool.device)
+        dtype = k_out.dtype
+        _need(k_out.shape[1] == heads and v_out.shape[1] == heads, "k_out and v_out have the cache's heads")
+        status = self.lib.padra_kv_read(
+            cache.ref, sequences.ref, k_out.data_ptr(), v_out.data_ptr(), _row_stride(k_out, rows, dim, dtype, "k_out"),
+            _row_stride(v_out, rows, dim, dtype, "v_out"), ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
+        if status:
+            raise B.PadraError(status, "padra_kv_read")
         return k_out, v_out
 
     def workspace(self, head_dim, stream):
-        """The workspace of calls on `stream` (a stream handle).  Made by the first call on the stream, which therefore comes
-        before any capture; captured calls keep using it, so graphs captured on one stream are not to be replayed side by side."""
-        key = stream, head_dim
-        if key not in self._workspace:
+        """(address, bytes) of the workspace of calls on `stream` (a stream handle): calls on one stream follow one another.  It is
+        made by the first call on the stream, which therefore comes before any capture; captured calls keep using it, so
+        graphs captured on one stream are not to be replayed side by side."""
+        found = self._workspace.get((stream, head_dim))
+        if found is None:
             _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
             n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
             ws = torch.empty(n, dtype=torch.uint8, device=self.bad.device)
-            self._workspace[key] = ws, ws.data_ptr(), n
-        return self._workspace[key][1:]
+            found = self._workspace[stream, head_dim] = ws.data_ptr(), n, ws
+        return found[:2]
 
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
         """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
-        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-        _need(q.shape[::2] == (sequences.rows, cache.head_dim) and out.shape == q.shape and out.dtype == q.dtype, "q and out are [rows][heads][head_dim] of one type")
-        handle = B.stream_handle(stream)
-        B.check(self.lib.padra_attention_q4(cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _heads(q, "q"), _heads(out, "out"), q.shape[1],
-                                            ROWS_TYPE[q.dtype], scale, window, *self.workspace(cache.head_dim, handle), self._bad, handle),
-                "padra_attention_q4")
+        rows, dim, dtype, heads = sequences.rows, cache.head_dim, q.dtype, q.shape[1]
+        if out is None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _need(out.shape[1] == heads, "out has as many heads as q")
+        stream = self._stream(stream)
+        status = self.lib.padra_attention_q4(
+            cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(out, rows, dim, dtype, "out"), heads,
+            ROWS_TYPE.get(dtype, -1), scale, window, *self.workspace(dim, stream), self._bad, stream)
+        if status:
+            raise B.PadraError(status, "padra_attention_q4")
         return out
