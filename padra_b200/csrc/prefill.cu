@@ -36,6 +36,7 @@
 #include "common.cuh"
 #include "exchange.cuh"
 #include "kernels.cuh"
+#include "tensor_memory.cuh"
 
 namespace padra {
 namespace {
@@ -60,7 +61,6 @@ constexpr int kMaxPairs = 4096 * kTopK;              // grouped pairs (rows) one
 constexpr int kMaxPairIndex = 1 << 20;              // pair indices may be sparse (received rows in per-source regions)
 constexpr int kMaxTiles = kExperts + kMaxPairs / kMaxTileN; // sum over experts of ceil(n_e / 256)
 constexpr int kAhead = 2;                           // own stages of packed words in flight per producer lane
-constexpr unsigned long long kWaitLimitNs = 1000000000ull; // a wait that lasts a second has failed
 constexpr int kMaxTokensPrefill = 2048;
 
 #ifdef PADRA_PREFILL_TRACE
@@ -115,101 +115,12 @@ struct PrefillArgs {
   unsigned epoch;
 };
 
-__device__ __forceinline__ unsigned SmemAddress(const void *p) {
-  return static_cast<unsigned>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void BarrierInit(unsigned long long *bar, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(SmemAddress(bar)), "r"(count) : "memory");
-}
-__device__ __forceinline__ void BarrierArrive(unsigned long long *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(SmemAddress(bar)) : "memory");
-}
-// Bounded wait for the phase of parity `parity`; false if it did not complete in time or the CTA is aborting.
-// `backoff` (nanoseconds of sleep after a failed poll) keeps warps with long waits off the issue slots the producers
-// need; the MMA thread polls without sleeping.
-__device__ __forceinline__ bool BarrierWait(unsigned long long *bar, unsigned parity, const volatile int *abort, unsigned backoff) {
-  const unsigned addr = SmemAddress(bar);
-  unsigned long long started = 0;
-  for (unsigned spins = 0;; ++spins) {
-    unsigned done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(done)
-                 : "r"(addr), "r"(parity)
-                 : "memory");
-    if (done)
-      return true;
-    if ((spins & 63u) == 63u) {
-      if (*abort)
-        return false;
-      unsigned long long now;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-      if (!started)
-        started = now;
-      else if (now - started > kWaitLimitNs)
-        return false;
-    }
-    if (backoff)
-      __nanosleep(backoff);
-  }
-}
-// K-major with 128-byte swizzle: rows of 128 bytes, eight-row groups 1024 bytes apart; a K16 step inside the 64-input row
-// is selected by moving the start address 32 bytes on.  Bits: [0,14) address>>4, [16,30) leading offset>>4 (unused
-// here), [32,46) distance between eight-row groups>>4, [46,48) descriptor version 1 (sm_100), [61,64) layout 2 =
-// SWIZZLE_128B.
-__device__ __forceinline__ unsigned long long SwizzledOperandDescriptor(unsigned smem_address) {
-  return static_cast<unsigned long long>((smem_address & 0x3ffffu) >> 4) | (1ull << 16) | (static_cast<unsigned long long>(1024 >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
-}
 // One tile of the 2-D tensor behind `map` (inner coordinate x in elements, a multiple of 8; outer coordinate y) into
 // shared memory; its bytes are counted on `bar`.  The CTA is the only reader of the tile.
 __device__ __forceinline__ void TensorTileLoad(void *smem, const CUtensorMap *map, int x, int y, unsigned long long *bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
                    SmemAddress(smem)),
                "l"(map), "r"(x), "r"(y), "r"(SmemAddress(bar))
-               : "memory");
-}
-__device__ __forceinline__ void BarrierExpect(unsigned long long *bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(SmemAddress(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ unsigned InstructionDescriptor(int n) {
-  // kind::f16: FP32 accumulate (bits 4-5 = 1), A and B FP16 (0), both K-major (0), N>>3 at [17,23), M>>4 at [24,29)
-  return (1u << 4) | (static_cast<unsigned>(n >> 3) << 17) | (static_cast<unsigned>(128 >> 4) << 24);
-}
-__device__ __forceinline__ void MmaSS(unsigned tmem_d, unsigned long long a_desc, unsigned long long b_desc, unsigned idesc, bool accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-               "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
-               : "memory");
-}
-__device__ __forceinline__ void MmaCommit(unsigned long long *bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(SmemAddress(bar)) : "memory");
-}
-// 32 lanes x 32 columns: thread i of the warp gets columns [column, column+32) of its own lane
-__device__ __forceinline__ void TmemLoad32(unsigned taddr, float (&v)[32]) {
-  unsigned r[32];
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-                 "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-                 "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-               : "r"(taddr)
-               : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i)
-    v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void TmemStore32(unsigned taddr, const float (&v)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-               "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-               "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])),
-               "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])),
-               "r"(__float_as_uint(v[8])), "r"(__float_as_uint(v[9])), "r"(__float_as_uint(v[10])), "r"(__float_as_uint(v[11])),
-               "r"(__float_as_uint(v[12])), "r"(__float_as_uint(v[13])), "r"(__float_as_uint(v[14])), "r"(__float_as_uint(v[15])),
-               "r"(__float_as_uint(v[16])), "r"(__float_as_uint(v[17])), "r"(__float_as_uint(v[18])), "r"(__float_as_uint(v[19])),
-               "r"(__float_as_uint(v[20])), "r"(__float_as_uint(v[21])), "r"(__float_as_uint(v[22])), "r"(__float_as_uint(v[23])),
-               "r"(__float_as_uint(v[24])), "r"(__float_as_uint(v[25])), "r"(__float_as_uint(v[26])), "r"(__float_as_uint(v[27])),
-               "r"(__float_as_uint(v[28])), "r"(__float_as_uint(v[29])), "r"(__float_as_uint(v[30])), "r"(__float_as_uint(v[31]))
                : "memory");
 }
 // four pieces x 8 columns: v[q][j] = column 32*q + j of the thread's lane, counted from `taddr`
