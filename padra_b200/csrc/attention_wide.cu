@@ -23,23 +23,30 @@ namespace attention {
 namespace {
 
 constexpr int kTile = 128, kColumns = 256;
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 8, kMmaWarp = kSoftmaxWarps + kProducerWarps, kWarps = kMmaWarp + 1, kThreads = kWarps * 32;
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 8, kMmaWarp = kSoftmaxWarps + kProducerWarps;
+constexpr int kWarps = kMmaWarp + 4, kThreads = kWarps * 32; // whole warpgroups, for the register split; three warps idle
+// Registers per thread: launched with 96 (640 threads), then split 2 * 120 + 2 * 88 + 64 = 5 * 96.
+constexpr int kSoftmaxRegisters = 120, kProducerRegisters = 88, kMmaRegisters = 64;
 constexpr int kStages = 2;
 
-template <int D> struct Smem {
-  static constexpr int kHalves = D / 64;
-  alignas(1024) unsigned char q[2][kHalves][128 * 128]; // rows of 64 values (128 bytes), 16-byte pieces swizzled by row
-  alignas(1024) unsigned char k[kStages][kHalves][kTile * 128];
-  alignas(1024) unsigned char v[kStages][kHalves][kTile * 128];
-  alignas(8) unsigned long long q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
-  unsigned long long shared_ready, shared_done; // the second half's maximum and sum are there / have been used
-  float2 other[128];
-  int item_begin[kThreads];
-  long long scan[kWarps], start_offset;
-  int start_sequence, start_block;
-  unsigned tmem;
-  int abort;
+// place / group and its remainder inside a unit: `reciprocal` = ceil(2^32 / group) gives the quotient exactly while
+// place * group < 2^32, which places counted from the block's first row (below group + 256, group at most 4096) keep to.
+struct Places {
+  int row0, rest0; // row and head of the block's first column
+  unsigned reciprocal;
+  int group;
+  __device__ __forceinline__ void Split(int column, int *row, int *head) const {
+    const unsigned x = static_cast<unsigned>(rest0 + column);
+    const int quotient = group == 1 ? static_cast<int>(x) : static_cast<int>(__umulhi(x, reciprocal));
+    *row = row0 + quotient, *head = static_cast<int>(x) - quotient * group;
+  }
 };
+__device__ __forceinline__ Places PlacesOf(const AttentionArgs &a, int block) {
+  Places p;
+  p.row0 = block * kColumns / a.group, p.rest0 = block * kColumns - p.row0 * a.group, p.group = a.group;
+  p.reciprocal = static_cast<unsigned>((0x100000000ull + a.group - 1) / static_cast<unsigned>(a.group));
+  return p;
+}
 
 // Blocks of a sequence, and what one of them asks for.
 struct Rows {
@@ -96,11 +103,56 @@ struct Walk {
   __device__ __forceinline__ bool Paired() const { return unit.columns <= 128; }
 };
 
-// One lane polls for its warp: true for all lanes or for none.
+template <int D> struct Smem {
+  static constexpr int kHalves = D / 64;
+  alignas(1024) unsigned char q[2][kHalves][128 * 128]; // rows of 64 values (128 bytes), 16-byte pieces swizzled by row
+  alignas(1024) unsigned char k[kStages][kHalves][kTile * 128];
+  alignas(1024) unsigned char v[kStages][kHalves][kTile * 128];
+  alignas(8) unsigned long long q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
+  unsigned long long q_empty;
+  unsigned long long shared_ready, shared_done; // the second half's maximum and sum are there / have been used
+  struct {
+    float factor; // what a column's scores are multiplied by
+    int last;     // its position: the last token it sees (-1: none)
+  } column[2][kColumns]; // of this piece and of the next
+  alignas(16) unsigned char out[kSoftmaxWarps][32 * 64]; // a warp's rows on their way out, 32 values at a time
+  float2 other[128];
+  int item_begin[kThreads];
+  long long scan[kWarps], start_offset;
+  int start_sequence, start_block;
+  Walk walk[kMmaWarp + 1]; // every working warp's place in the run: in registers it crowded out what the loops need
+  unsigned tmem;
+  int abort;
+};
+
+// Bounded wait (see BarrierWait) that lets the hardware suspend the thread for up to two microseconds at a time: seventeen warps wait
+// here most of the time, and plain polling took issue slots from the ones at work.
+__device__ __forceinline__ bool SuspendedWait(unsigned long long *bar, unsigned parity, const volatile int *abort) {
+  const unsigned address = SmemAddress(bar);
+  unsigned long long started = 0;
+  for (;;) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(address), "r"(parity), "r"(2000u)
+                 : "memory");
+    if (done)
+      return true;
+    if (*abort)
+      return false;
+    unsigned long long now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    if (!started)
+      started = now;
+    else if (now - started > kWaitLimitNs)
+      return false;
+  }
+}
+// One lane waits for its warp: true for all lanes or for none.
 __device__ __forceinline__ bool WarpWait(unsigned long long *bar, unsigned parity, const volatile int *abort) {
   int done = 0;
   if ((threadIdx.x & 31) == 0)
-    done = BarrierWait(bar, parity, abort, 0);
+    done = SuspendedWait(bar, parity, abort);
   return __shfl_sync(0xffffffffu, done, 0) != 0;
 }
 __device__ __forceinline__ void FenceToTensorCores() { // this thread's shared-memory writes before the tensor cores' reads
@@ -122,10 +174,49 @@ __device__ __forceinline__ void MmaTS(unsigned tmem_d, unsigned tmem_a, unsigned
                : "memory");
 }
 __device__ __forceinline__ void TmemStore16(unsigned taddr, const unsigned (&v)[16]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
-               "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+               "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                : "memory");
+}
+__device__ __forceinline__ void TmemStore32(unsigned taddr, const unsigned (&v)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+               "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+               "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+               "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+               : "memory");
+}
+// Columns of the thread's lane.
+__device__ __forceinline__ void TmemLoad16(unsigned taddr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                 "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    asm volatile("" : "+f"(v[i])); // no use of a value moves up across the wait
+}
+__device__ __forceinline__ void TmemLoad64(unsigned taddr, float (&v)[64]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                 "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                 "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+                 "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+                 "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+                 "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+                 "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+                 "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i)
+    asm volatile("" : "+f"(v[i])); // no use of a value moves up across the wait
 }
 __device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -184,55 +275,92 @@ template <int D> struct Producer {
 };
 
 // ---- softmax ----
-template <typename T, int D> struct Column { // one query column of a block
-  float factor, top, sum;
-  int first, last; // tokens it sees
-};
-
-// Stages one query row as FP16 (divided by a power of two, times the sign of scale) into row `row` of a half's Q tile.
-template <typename T, int D>
-__device__ __forceinline__ void StageQuery(const AttentionArgs &a, const Rows &r, int head, int place, bool there, unsigned char *tile, int row,
-                                           Column<T, D> *to) {
-  const int sequence_row = place / a.group, h = head * a.group + place % a.group, position = r.context - r.rows + sequence_row;
-  const bool load = there && position >= 0;
-  const T *const from = static_cast<const T *>(a.q) + static_cast<long long>(r.begin + sequence_row) * a.q_stride + h * D;
-  uint4 raw[D / 8];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i)
-    raw[i] = load ? *reinterpret_cast<const uint4 *>(from + 8 * i) : make_uint4(0, 0, 0, 0);
-  float most = 0;
-  bool finite = true;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    float x[8];
-    Widen(raw[i], from, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      finite &= isfinite(x[j]) != 0;
-      most = fmaxf(most, fabsf(x[j]));
-    }
-  }
-  if (!finite)
-    Raise(a.bad);
-  const int exponent = most > 0 && finite ? min(126, max(-126, ilogbf(most))) : 0;
-  const float shrink = finite ? ldexpf(a.sign, -exponent) : 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) {
-    float x[8];
-    Widen(raw[i], from, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[j] = finite ? x[j] * shrink : 0.f;
-    *reinterpret_cast<uint4 *>(tile + PieceOffset(row, i)) = make_uint4(Pack(x[0], x[4]), Pack(x[1], x[5]), Pack(x[2], x[6]), Pack(x[3], x[7]));
-  }
-  to->factor = a.scale * ldexpf(1.f, exponent), to->top = kNever, to->sum = 0;
-  to->last = there && finite ? position : -1;
-  to->first = a.window ? max(0, to->last - a.window + 1) : 0;
+__device__ __forceinline__ float2 Fma2(float2 x, float2 y, float2 z) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
+  return r;
+}
+__device__ __forceinline__ float2 Add2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
+  return r;
+}
+__device__ __forceinline__ float Max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
 }
 
-// Smallest `last` and largest `first` over the warp's columns that exist: a tile inside them needs no mask.
-__device__ __forceinline__ int WarpMin(int x) { return __reduce_min_sync(0xffffffffu, x); }
-__device__ __forceinline__ int WarpMax(int x) { return __reduce_max_sync(0xffffffffu, x); }
+// ---- queries ----
+// 2^exponent of a float's leading bit, and the reciprocal (finite, in the normal range of both)
+__device__ __forceinline__ float PowerOf(float x) {
+  return __uint_as_float(min(max(__float_as_uint(x) & 0x7f800000u, 1u << 23), 253u << 23));
+}
+__device__ __forceinline__ float ReciprocalPower(float power) {
+  return __uint_as_float((254u << 23) - __float_as_uint(power));
+}
+
+// Stages the query rows of 32 columns of a block (column0 ..., those below `columns`) as FP16, divided by a power of two and times the
+// sign of scale, into a half's Q tile (rows column0 % 128 ...), and notes their factors and positions.  D / 8 lanes read a row together.
+template <typename T, int D>
+__device__ __forceinline__ void StageQueries(const AttentionArgs &a, const Rows &r, int head, const Places &places, int column0, int columns, Smem<D> &sm,
+                                             int parity) {
+  constexpr int kLanes = D / 8, kSide = 32 / kLanes, kFlight = 4;
+  const int lane = threadIdx.x & 31, side = lane / kLanes, piece = lane % kLanes;
+  const int start = r.context - r.rows;
+  unsigned char *const tile = sm.q[column0 >> 7][0];
+#pragma unroll 1
+  for (int c0 = column0; c0 < column0 + 32; c0 += kSide * kFlight) {
+    uint4 raw[kFlight];
+    int position[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int c = c0 + f * kSide + side;
+      int row, h;
+      places.Split(c, &row, &h);
+      position[f] = start + row;
+      raw[f] = c < columns && position[f] >= 0
+                   ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + static_cast<long long>(r.begin + row) * a.q_stride +
+                                                           (head * a.group + h) * D + 8 * piece))
+                   : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int c = c0 + f * kSide + side;
+      float x[8], most = 0;
+      Widen(raw[f], static_cast<const T *>(nullptr), x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) // as integers: an exponent of all ones (infinity, NaN) is larger than everything else
+        most = __uint_as_float(max(__float_as_uint(most), __float_as_uint(x[j]) & 0x7fffffffu));
+      unsigned bits = __float_as_uint(most);
+#pragma unroll
+      for (int m = 1; m < kLanes; m *= 2)
+        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, m));
+      const bool finite = bits < 0x7f800000u;
+      const float power = PowerOf(__uint_as_float(bits)), shrink = finite ? ReciprocalPower(power) * a.sign : 0.f;
+      if (finite) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[j] *= shrink;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[j] = 0;
+      }
+      *reinterpret_cast<uint4 *>(tile + PieceOffset(c & 127, piece)) = make_uint4(Pack(x[0], x[4]), Pack(x[1], x[5]), Pack(x[2], x[6]), Pack(x[3], x[7]));
+      if (piece == 0) {
+        if (!finite)
+          Raise(a.bad);
+        sm.column[parity][c].factor = a.scale * (finite ? power : 1.f);
+        sm.column[parity][c].last = c < columns && finite ? position[f] : -1;
+      }
+    }
+  }
+}
 
 template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) WideAttentionKernel(const __grid_constant__ AttentionArgs a) {
   using S = Smem<D>;
@@ -282,13 +410,14 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     a.split[blockIdx.x].pieces = 0;
     sm.abort = 0;
     for (int i = 0; i < 2; ++i) {
-      BarrierInit(&sm.q_full[i], kSoftmaxWarps / 2), BarrierInit(&sm.s_full[i], 1);
+      BarrierInit(&sm.q_full[i], kProducerWarps / 2), BarrierInit(&sm.s_full[i], 1);
       BarrierInit(&sm.p_full[i], kSoftmaxWarps / 2), BarrierInit(&sm.o_full[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       BarrierInit(&sm.k_full[i], kProducerWarps), BarrierInit(&sm.v_full[i], kProducerWarps);
       BarrierInit(&sm.k_empty[i], 1), BarrierInit(&sm.v_empty[i], 1);
     }
+    BarrierInit(&sm.q_empty, 1);
     BarrierInit(&sm.shared_ready, kSoftmaxWarps / 2), BarrierInit(&sm.shared_done, kSoftmaxWarps / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -309,70 +438,96 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
   AfterSync();
   const unsigned tmem = sm.tmem;
   const volatile int *const abort = &sm.abort;
-  Walk walk;
-  walk.Begin(a, begin, end, sm.start_sequence, sm.start_block, sm.start_offset);
+  Walk &walk = sm.walk[min(warp, kMmaWarp)];
+  if (lane == 0 && warp <= kMmaWarp)
+    walk.Begin(a, begin, end, sm.start_sequence, sm.start_block, sm.start_offset);
+  __syncwarp();
+  auto next_piece = [&]() { // by the whole warp
+    __syncwarp();
+    if (lane == 0)
+      walk.Next(a);
+    __syncwarp();
+  };
   bool alive = true;
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
     // =============================== producers ===============================
     using P = Producer<D>;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
     const int mine = 16 * (warp - kSoftmaxWarps), chunk = lane % P::kChunks; // this warp's tokens of a tile
-    Walk ahead = walk; // the piece of the tile that is loaded next
-    int ahead_tile = 0;
-    P next;
-    int next_page = -1;
-    auto low_of = [&](const Walk &w) { // first token that some column of the unit sees
-      return a.window ? max(0, w.rows.context - w.rows.rows + w.block * kColumns / a.group + 1 - a.window) : 0;
-    };
-    auto find = [&]() { // the page of the warp's tokens in the tile at `ahead`
-      next_page = -1;
-      if (ahead.More()) {
-        const int t = (ahead.unit.first + ahead.skip + ahead_tile) * kTile + mine;
-        if (t < ahead.rows.context && t + 16 > low_of(ahead))
-          next_page = PageOf(a.seq, a.cache, ahead.s, t, a.bad);
+    int tile = 0, page = -1; // of the piece: the tile that is loaded next, and the page of the warp's tokens in it
+    P data;
+    auto find = [&]() {
+      page = -1;
+      if (walk.More()) {
+        const int t = (walk.unit.first + walk.skip + tile) * kTile + mine;
+        // first token that some column of the unit sees
+        const int low = a.window ? max(0, walk.rows.context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
+        if (t < walk.rows.context && t + 16 > low)
+          page = PageOf(a.seq, a.cache, walk.s, t, a.bad);
       }
     };
+    // A piece's queries come before its first tile: this warp's 32 columns, once the MMAs of the piece before are done with Q.
+    unsigned pieces = 0;
+    auto stage_queries = [&]() {
+      const int column0 = 32 * (warp - kSoftmaxWarps);
+      if (pieces && !(alive = WarpWait(&sm.q_empty, (pieces - 1) & 1, abort)))
+        return;
+      if (column0 < 128 || !walk.Paired()) {
+        StageQueries<T, D>(a, walk.rows, walk.head, PlacesOf(a, walk.block), column0, walk.unit.columns, sm, pieces & 1);
+        FenceToTensorCores();
+        __syncwarp();
+        if (lane == 0)
+          BarrierArrive(&sm.q_full[column0 >> 7]);
+      }
+      ++pieces;
+    };
     auto load = [&]() { // that tile's codes, then the page of the one after it
-      if (ahead.More()) {
-        next.Load(a, next_page, ahead.head, (ahead.unit.first + ahead.skip + ahead_tile) * kTile + mine, ahead.rows.context);
-        if (++ahead_tile == ahead.count)
-          ahead.Next(a), ahead_tile = 0;
+      if (walk.More()) {
+        data.Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, walk.rows.context);
+        if (++tile == walk.count)
+          next_piece(), tile = 0;
         find();
       }
     };
     find();
+    stage_queries();
     load();
-    for (unsigned n = 0; alive && walk.More(); walk.Next(a))
-      for (int i = 0; i < walk.count; ++i, ++n) {
-        const P now = next;
-        load();
-        const int stage = n & (kStages - 1);
-        const unsigned free_parity = ((n / kStages) & 1) ^ 1;
-        alive = WarpWait(&sm.k_empty[stage], free_parity, abort);
-        if (!alive)
-          break;
+    const unsigned tiles = static_cast<unsigned>(end - begin);
+    for (unsigned n = 0; n < tiles && alive; ++n) {
+      const int stage = n & (kStages - 1);
+      const unsigned free_parity = ((n / kStages) & 1) ^ 1;
+      alive = WarpWait(&sm.k_empty[stage], free_parity, abort);
+      if (!alive)
+        break;
 #pragma unroll
-        for (int j = 0; j < P::kTokens; ++j)
-          P::Store(sm.k[stage][0], mine + P::TokenOf(lane, j), chunk, now.k[j], now.k_scale[j]);
-        FenceToTensorCores();
-        __syncwarp();
-        if (lane == 0)
-          BarrierArrive(&sm.k_full[stage]);
-        alive = WarpWait(&sm.v_empty[stage], free_parity, abort);
-        if (!alive)
-          break;
+      for (int j = 0; j < P::kTokens; ++j)
+        P::Store(sm.k[stage][0], mine + P::TokenOf(lane, j), chunk, data.k[j], data.k_scale[j]);
+      FenceToTensorCores();
+      __syncwarp();
+      if (lane == 0)
+        BarrierArrive(&sm.k_full[stage]);
+      alive = WarpWait(&sm.v_empty[stage], free_parity, abort);
+      if (!alive)
+        break;
 #pragma unroll
-        for (int j = 0; j < P::kTokens; ++j)
-          P::Store(sm.v[stage][0], mine + P::TokenOf(lane, j), chunk, now.v[j], now.v_scale[j]);
-        FenceToTensorCores();
-        __syncwarp();
-        if (lane == 0)
-          BarrierArrive(&sm.v_full[stage]);
+      for (int j = 0; j < P::kTokens; ++j)
+        P::Store(sm.v[stage][0], mine + P::TokenOf(lane, j), chunk, data.v[j], data.v_scale[j]);
+      FenceToTensorCores();
+      __syncwarp();
+      if (lane == 0)
+        BarrierArrive(&sm.v_full[stage]);
+      if (n + 1 < tiles) {
+        if (tile == 0) // the next tile begins a piece
+          stage_queries();
+        load(); // arrives while the MMAs free the next stage
       }
-  } else if (warp == kMmaWarp) {
+    }
+  } else if (warp >= kMmaWarp) {
     // =============================== MMA issue ===============================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
     // Job i of a piece: half i & 1 with tile i / 2, or with tile i where both halves work on the same columns.
-    if (lane == 0) {
+    if (warp == kMmaWarp && lane == 0) {
       const unsigned s_desc = InstructionDescriptor(kTile), o_desc = InstructionDescriptor(D) | kSecondOperandRowMajor;
       unsigned tiles = 0, jobs_of[2] = {0, 0}, pieces_of[2] = {0, 0}; // all so far: tiles, jobs and staged Q tiles of the halves
       for (; alive && walk.More(); walk.Next(a)) {
@@ -381,7 +536,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         auto scores = [&](int i) { // S of job i
           const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
           if (paired || half == 0)
-            if (!(alive = BarrierWait(&sm.k_full[stage], ((tiles + tile) / kStages) & 1, abort, 0)))
+            if (!(alive = SuspendedWait(&sm.k_full[stage], ((tiles + tile) / kStages) & 1, abort)))
               return;
           AfterSync();
           const unsigned q_address = SmemAddress(sm.q[paired ? 0 : half][0]), k_address = SmemAddress(sm.k[stage][0]);
@@ -393,21 +548,23 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           MmaCommit(&sm.s_full[half]);
           if (paired || half == 1)
             MmaCommit(&sm.k_empty[stage]);
+          if (i == jobs - 1)
+            MmaCommit(&sm.q_empty);
         };
         // Q of this piece: the second half's tile is staged only where it has columns of its own
-        alive = BarrierWait(&sm.q_full[0], pieces_of[0]++ & 1, abort, 0);
+        alive = SuspendedWait(&sm.q_full[0], pieces_of[0]++ & 1, abort);
         if (alive)
           scores(0);
         if (alive && !paired)
-          alive = BarrierWait(&sm.q_full[1], pieces_of[1]++ & 1, abort, 0);
+          alive = SuspendedWait(&sm.q_full[1], pieces_of[1]++ & 1, abort);
         if (alive && jobs > 1)
           scores(1);
         for (int i = 0; i < jobs && alive; ++i) {
           const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
           if (paired || half == 0)
-            if (!(alive = BarrierWait(&sm.v_full[stage], ((tiles + tile) / kStages) & 1, abort, 0)))
+            if (!(alive = SuspendedWait(&sm.v_full[stage], ((tiles + tile) / kStages) & 1, abort)))
               break;
-          if (!(alive = BarrierWait(&sm.p_full[half], jobs_of[half]++ & 1, abort, 0)))
+          if (!(alive = SuspendedWait(&sm.p_full[half], jobs_of[half]++ & 1, abort)))
             break;
           AfterSync();
           const unsigned v_address = SmemAddress(sm.v[stage][0]);
@@ -432,86 +589,96 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     __syncwarp();
   } else {
     // =============================== softmax ===============================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int half = warp / 4, row = tid & 127; // the thread's column of its half, and its lane in tensor memory
     const unsigned lanes = static_cast<unsigned>((warp & 3) * 32) << 16, s_address = tmem + lanes + 128 * half, o_address = tmem + lanes + 256 + 128 * half;
-    unsigned jobs = 0, finished[2] = {0, 0}, shared = 0; // phases gone by: S tiles, outputs of the halves, joined pieces
-    for (; alive && walk.More(); walk.Next(a)) {
+    unsigned jobs = 0, staged[2] = {0, 0}, finished[2] = {0, 0}, shared = 0, pieces = 0; // phases gone by: S, Q, outputs of the halves, joins
+    for (; alive && walk.More(); next_piece(), ++pieces) {
       const bool paired = walk.Paired();
-      const int own = paired ? row : 128 * half + row, place = walk.block * kColumns + own;
+      const int own = paired ? row : 128 * half + row; // column of the block
       const bool there = own < walk.unit.columns;
-      Column<T, D> column;
-      // where both halves work on the same columns, the first one stages them; the second needs the numbers only
-      StageQuery<T, D>(a, walk.rows, walk.head, place, there, sm.q[half][0], row, &column);
-      FenceToTensorCores();
-      __syncwarp();
-      if (lane == 0 && !(paired && half))
-        BarrierArrive(&sm.q_full[half]);
-      const int least = WarpMin(there ? column.last : 0x7fffffff), latest = WarpMax(there ? column.first : 0);
+      // the block's columns are staged by the producers, those that both halves work on once
+      if (paired || !half) {
+        alive = WarpWait(&sm.q_full[0], staged[0]++ & 1, abort);
+        staged[1] += !paired;
+      } else {
+        ++staged[0];
+        alive = WarpWait(&sm.q_full[1], staged[1]++ & 1, abort);
+      }
+      if (!alive)
+        break;
+      const float factor = sm.column[pieces & 1][own].factor;
+      const int last = sm.column[pieces & 1][own].last, first = a.window ? max(0, last - a.window + 1) : 0;
+      float top = kNever, total = 0;
+      const int least = __reduce_min_sync(0xffffffffu, there ? last : 0x7fffffff), latest = __reduce_max_sync(0xffffffffu, there ? first : 0);
       const int first_tile = walk.unit.first + walk.skip;
       const int step = paired ? 2 : 1, begin_tile = paired ? half : 0;
       for (int i = begin_tile; i < walk.count; i += step, ++jobs) {
         const int t0 = (first_tile + i) * kTile;
-        const bool edge = t0 + kTile - 1 > least || t0 < latest; // some column does not see all of the tile
         alive = WarpWait(&sm.s_full[half], jobs & 1, abort);
         if (!alive)
           break;
         AfterSync();
-        float most = -INFINITY;
+        if (t0 + kTile - 1 > least || t0 < latest) { // some column does not see all of the tile: masked in place
+#pragma unroll 1
+          for (int piece = 0; piece < kTile / 16; ++piece) {
+            float x[16];
+            unsigned y[16];
+            TmemLoad16(s_address + 16 * piece, x);
 #pragma unroll
-        for (int piece = 0; piece < 4; ++piece) {
-          float x[32];
-          TmemLoad32(s_address + 32 * piece, x);
-          if (edge) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int t = t0 + 32 * piece + j;
-              x[j] = t < column.first || t > column.last ? -INFINITY : x[j];
+            for (int j = 0; j < 16; ++j) {
+              const int t = t0 + 16 * piece + j;
+              y[j] = t < first || t > last ? 0xff800000u : __float_as_uint(x[j]);
             }
+            TmemStore16(s_address + 16 * piece, y);
           }
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            most = fmaxf(most, x[j]);
+          TmemStoreWait();
         }
-        const bool raise = fmaf(most, column.factor, -column.top) > kRaise;
+        float most = -INFINITY;
+#pragma unroll 1
+        for (int piece = 0; piece < 2; ++piece) {
+          float x[64];
+          TmemLoad64(s_address + 64 * piece, x);
+          float part[2] = {most, x[0]};
+#pragma unroll
+          for (int j = 0; j < 64; j += 2)
+            part[j >> 1 & 1] = Max3(part[j >> 1 & 1], x[j], x[j + 1]);
+          most = fmaxf(part[0], part[1]);
+        }
+        const bool raise = fmaf(most, factor, -top) > kRaise;
         if (__any_sync(0xffffffffu, raise)) {
-          const float next = raise ? fmaf(most, column.factor, -kTop) : column.top, shrink = Exp2(column.top - next);
-          column.top = next, column.sum *= shrink;
+          const float next = raise ? fmaf(most, factor, -kTop) : top, shrink = Exp2(top - next);
+          top = next, total *= shrink;
           if (i != begin_tile) { // the S that has just come says that the MMAs before it are done with O
 #pragma unroll 1
-            for (int piece = 0; piece < D / 32; ++piece) {
-              float x[32];
-              TmemLoad32(o_address + 32 * piece, x);
+            for (int piece = 0; piece < D / 16; ++piece) {
+              float y[16];
+              TmemLoad16(o_address + 16 * piece, y);
+              unsigned z[16];
 #pragma unroll
-              for (int j = 0; j < 32; ++j)
-                x[j] *= shrink;
-              TmemStore32(o_address + 32 * piece, x);
+              for (int j = 0; j < 16; ++j)
+                z[j] = __float_as_uint(y[j] * shrink);
+              TmemStore16(o_address + 16 * piece, z);
             }
           }
         }
-        float sum = 0;
+        const float2 factors = make_float2(factor, factor), minus_top = make_float2(-top, -top);
+        float2 sum[2] = {make_float2(total, 0), make_float2(0, 0)};
+#pragma unroll 1
+        for (int piece = 0; piece < 2; ++piece) {
+          float x[64];
+          TmemLoad64(s_address + 64 * piece, x);
+          unsigned packed[32];
 #pragma unroll
-        for (int piece = 0; piece < 4; ++piece) {
-          float x[32];
-          TmemLoad32(s_address + 32 * piece, x);
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            x[j] = Exp2(fmaf(x[j], column.factor, -column.top));
-          if (edge) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int t = t0 + 32 * piece + j;
-              x[j] = t < column.first || t > column.last ? 0.f : x[j];
-            }
+          for (int j = 0; j < 32; ++j) {
+            const float2 e = Fma2(make_float2(x[2 * j], x[2 * j + 1]), factors, minus_top), p = make_float2(Exp2(e.x), Exp2(e.y));
+            sum[j & 1] = Add2(sum[j & 1], p);
+            packed[j] = Pack(p.x, p.y);
           }
-          unsigned packed[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            sum += x[2 * j] + x[2 * j + 1];
-            packed[j] = Pack(x[2 * j], x[2 * j + 1]);
-          }
-          TmemStore16(s_address + 16 * piece, packed); // over scores that have been read
+          TmemStore32(s_address + 32 * piece, packed); // over scores that have been read
         }
-        column.sum += sum;
+        sum[0] = Add2(sum[0], sum[1]);
+        total = sum[0].x + sum[0].y;
         TmemStoreWait();
         BeforeSync();
         __syncwarp();
@@ -522,10 +689,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         break;
       // ---- the piece's output ----
       const bool other_half = paired && walk.count > 1; // the second half has had tiles of these columns
-      float own_weight = 1.f, other_weight = 0.f;
       if (paired && half) {
         if (other_half) {
-          sm.other[row] = make_float2(column.top, column.sum);
+          sm.other[row] = make_float2(top, total);
           __syncwarp();
           if (lane == 0)
             BarrierArrive(&sm.shared_ready);
@@ -535,14 +701,15 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         }
         continue;
       }
+      float own_weight = 1.f, other_weight = 0.f;
       if (other_half) {
         alive = WarpWait(&sm.shared_ready, shared++ & 1, abort) && WarpWait(&sm.o_full[1], finished[1]++ & 1, abort);
         if (!alive)
           break;
         const float2 other = sm.other[row];
-        const float top = fmaxf(column.top, other.x);
-        own_weight = Exp2(column.top - top), other_weight = Exp2(other.x - top);
-        column.top = top, column.sum = own_weight * column.sum + other_weight * other.y;
+        const float larger = fmaxf(top, other.x);
+        own_weight = Exp2(top - larger), other_weight = Exp2(other.x - larger);
+        top = larger, total = own_weight * total + other_weight * other.y;
       }
       if (!paired && !half)
         ++finished[1]; // an output that is not this half's business
@@ -553,10 +720,13 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       const bool whole = walk.count == walk.unit.tiles;
       const int slot = walk.at == begin ? 0 : 1;
       float *const partial = PartialOf<D, kColumns>(a, blockIdx.x, slot);
-      const float inverse = whole ? (column.sum > 0 ? 1.f / column.sum : 0.f) : 1.f;
+      const float inverse = whole ? (total > 0 ? 1.f / total : 0.f) : 1.f;
       own_weight *= inverse, other_weight *= inverse;
-      const int sequence_row = place / a.group, h = walk.head * a.group + place % a.group;
-      T *const out = static_cast<T *>(a.out) + static_cast<long long>(walk.rows.begin + sequence_row) * a.out_stride + h * D;
+      // Rows of a whole unit go out 32 values at a time through shared memory, four lanes to a row.  Blocks of eight values lie in
+      // the order 0 4 1 5 2 6 3 7.
+      const Places places = PlacesOf(a, walk.block);
+      unsigned char *const out = sm.out[warp];
+      const int warp_there = walk.unit.columns - (own - lane); // columns of this warp that exist, if less than 32
 #pragma unroll 1
       for (int piece = 0; piece < D / 32; ++piece) {
         float x[32];
@@ -571,17 +741,29 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           for (int j = 0; j < 32; ++j)
             x[j] = fmaf(y[j], other_weight, x[j]);
         }
-        if (there) { // blocks of eight lie in the order 0 4 1 5 2 6 3 7
 #pragma unroll
-          for (int b = 0; b < 32; b += 8) {
-            const float4 first = make_float4(x[b], x[b + 2], x[b + 4], x[b + 6]), second = make_float4(x[b + 1], x[b + 3], x[b + 5], x[b + 7]);
-            if (whole) {
-              Store4(out + 32 * piece + b, first), Store4(out + 32 * piece + b + 4, second);
-            } else {
-              *reinterpret_cast<float4 *>(partial + own * D + 32 * piece + b) = first;
-              *reinterpret_cast<float4 *>(partial + own * D + 32 * piece + b + 4) = second;
-            }
+        for (int b = 0; b < 32; b += 8) {
+          const float4 front = make_float4(x[b], x[b + 2], x[b + 4], x[b + 6]), back = make_float4(x[b + 1], x[b + 3], x[b + 5], x[b + 7]);
+          if (whole) {
+            unsigned char *const to = out + 64 * lane + 16 * ((b / 8) ^ ((lane >> 1) & 3));
+            Store4(reinterpret_cast<T *>(to), front), Store4(reinterpret_cast<T *>(to + 8), back);
+          } else if (there) {
+            *reinterpret_cast<float4 *>(partial + own * D + 32 * piece + b) = front;
+            *reinterpret_cast<float4 *>(partial + own * D + 32 * piece + b + 4) = back;
           }
+        }
+        if (whole) {
+          __syncwarp();
+#pragma unroll
+          for (int c = lane / 4; c < 32; c += 8)
+            if (c < warp_there) {
+              int sequence_row, h;
+              places.Split(own - lane + c, &sequence_row, &h);
+              *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + static_cast<long long>(walk.rows.begin + sequence_row) * a.out_stride +
+                                         (walk.head * a.group + h) * D + 32 * piece + 8 * (lane & 3)) =
+                  *reinterpret_cast<const uint4 *>(out + 64 * c + 16 * ((lane & 3) ^ ((c >> 1) & 3)));
+            }
+          __syncwarp();
         }
       }
       if (other_half) {
@@ -592,7 +774,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       }
       if (!whole) {
         if (there)
-          *reinterpret_cast<float2 *>(partial + kColumns * D + 2 * own) = make_float2(column.top, column.sum);
+          *reinterpret_cast<float2 *>(partial + kColumns * D + 2 * own) = make_float2(top, total);
         if (!walk.skip && tid == 0) { // the unit begins here and goes on in the next runs
           const long long last = Quotient(walk.at + walk.unit.tiles - 1, share);
           a.split[blockIdx.x] = Split{static_cast<int>(last - blockIdx.x) + 1, slot, walk.rows.begin, walk.block, walk.head, walk.unit.columns};
