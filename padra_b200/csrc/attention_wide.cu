@@ -161,16 +161,25 @@ __device__ __forceinline__ void FenceToTensorCores() { // this thread's shared-m
 __device__ __forceinline__ void BeforeSync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void AfterSync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// V: rows of 64 values, one per token; the contraction runs over rows.  Blocks of 64 output values are `leading` bytes apart,
-// groups of eight tokens 1024.
-__device__ __forceinline__ unsigned long long RowMajorOperandDescriptor(unsigned smem_address, unsigned leading) {
-  return static_cast<unsigned long long>((smem_address & 0x3ffffu) >> 4) | (static_cast<unsigned long long>(leading >> 4) << 16) |
-         (static_cast<unsigned long long>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// Operand descriptors (see SwizzledOperandDescriptor for the fields), low and high word apart: the steps of a tile differ in the low
+// word's address only, and one thread builds two descriptors per MMA.
+// K-major (Q, K): the leading offset is unused.  MN-major (V: rows of 64 values, one per token; the contraction runs over rows): blocks of 64
+// output values are 16 KB apart, groups of eight tokens 1024 bytes.
+constexpr unsigned kDescriptorHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ unsigned DescriptorLow(unsigned smem_address, unsigned leading) {
+  return ((smem_address & 0x3ffffu) >> 4) | (leading >> 4) << 16;
+}
+__device__ __forceinline__ void MmaStepSS(unsigned tmem_d, unsigned a_low, unsigned b_low, unsigned idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(tmem_d),
+               "r"(a_low), "r"(b_low), "r"(kDescriptorHigh), "r"(idesc), "r"(accumulate ? 1u : 0u)
+               : "memory");
 }
 constexpr unsigned kSecondOperandRowMajor = 1u << 16; // instruction descriptor: B is MN-major
-__device__ __forceinline__ void MmaTS(unsigned tmem_d, unsigned tmem_a, unsigned long long b_desc, unsigned idesc, bool accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-               "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u)
+__device__ __forceinline__ void MmaStepTS(unsigned tmem_d, unsigned tmem_a, unsigned b_low, unsigned idesc, bool accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(tmem_d),
+               "r"(tmem_a), "r"(b_low), "r"(kDescriptorHigh), "r"(idesc), "r"(accumulate ? 1u : 0u)
                : "memory");
 }
 __device__ __forceinline__ void TmemStore16(unsigned taddr, const unsigned (&v)[16]) {
@@ -539,11 +548,11 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
             if (!(alive = SuspendedWait(&sm.k_full[stage], ((tiles + tile) / kStages) & 1, abort)))
               return;
           AfterSync();
-          const unsigned q_address = SmemAddress(sm.q[paired ? 0 : half][0]), k_address = SmemAddress(sm.k[stage][0]);
+          const unsigned q_low = DescriptorLow(SmemAddress(sm.q[paired ? 0 : half][0]), 16), k_low = DescriptorLow(SmemAddress(sm.k[stage][0]), 16);
 #pragma unroll
           for (int step = 0; step < D / 16; ++step) {
-            const unsigned offset = (step >> 2) * (128 * 128) + (step & 3) * 32;
-            MmaSS(tmem + 128 * half, SwizzledOperandDescriptor(q_address + offset), SwizzledOperandDescriptor(k_address + offset), s_desc, step > 0);
+            const unsigned offset = ((step >> 2) * (128 * 128) + (step & 3) * 32) >> 4;
+            MmaStepSS(tmem + 128 * half, q_low + offset, k_low + offset, s_desc, step > 0);
           }
           MmaCommit(&sm.s_full[half]);
           if (paired || half == 1)
@@ -567,11 +576,10 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           if (!(alive = SuspendedWait(&sm.p_full[half], jobs_of[half]++ & 1, abort)))
             break;
           AfterSync();
-          const unsigned v_address = SmemAddress(sm.v[stage][0]);
+          const unsigned v_low = DescriptorLow(SmemAddress(sm.v[stage][0]), 128 * 128);
 #pragma unroll
           for (int step = 0; step < kTile / 16; ++step)
-            MmaTS(tmem + 256 + 128 * half, tmem + 128 * half + 8 * step, RowMajorOperandDescriptor(v_address + step * 2048, 128 * 128), o_desc,
-                  i > 1 || step > 0);
+            MmaStepTS(tmem + 256 + 128 * half, tmem + 128 * half + 8 * step, v_low + step * (2048 >> 4), o_desc, i > 1 || step > 0);
           if (paired || half == 1)
             MmaCommit(&sm.v_empty[stage]);
           if (i + 2 >= jobs)
