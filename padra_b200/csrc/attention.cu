@@ -231,7 +231,7 @@ template <typename T, int D, int NT> struct Piece {
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp(); // the tile is here for every lane, and nobody reads the slot that is filled next
       fetch(i + kStages - 1);
-      const unsigned char *const tile = own_ring + (i & (kStages - 1)) * TileBytes<D>::kAll;
+      const unsigned tile = ring_address + (i & (kStages - 1)) * TileBytes<D>::kAll;
       const int t0 = (first_tile + warp + i * kWarps) * kTile;
       const bool edge = t0 + kTile - 1 > least || t0 < latest_low;
 
@@ -244,15 +244,16 @@ template <typename T, int D, int NT> struct Piece {
         for (int r = 0; r < 2; ++r) {
           const int token = 16 * half + 8 * r + g;
           if constexpr (kGroups == 4) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(tile + token * (D / 2) + 16 * c);
+            const uint4 u = LoadShared16(tile + token * (D / 2) + 16 * c);
             w[r][0] = u.x, w[r][1] = u.y, w[r][2] = u.z, w[r][3] = u.w;
-            const uint2 v = *reinterpret_cast<const uint2 *>(tile + TileBytes<D>::kCodes + token * (D / 16));
+            const uint2 v = LoadShared8(tile + TileBytes<D>::kCodes + token * (D / 16));
             const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), f1 = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
             f[r][0] = f0.x, f[r][1] = f0.y, f[r][2] = f1.x, f[r][3] = f1.y;
           } else {
-            const uint2 u = *reinterpret_cast<const uint2 *>(tile + token * (D / 2) + 8 * c);
+            const uint2 u = LoadShared8(tile + token * (D / 2) + 8 * c);
             w[r][0] = u.x, w[r][1] = u.y;
-            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(tile + TileBytes<D>::kCodes + token * (D / 16)));
+            const unsigned v = LoadShared4(tile + TileBytes<D>::kCodes + token * (D / 16));
+            const float2 f0 = __half22float2(*reinterpret_cast<const __half2 *>(&v));
             f[r][0] = f0.x, f[r][1] = f0.y;
           }
         }
@@ -265,8 +266,8 @@ template <typename T, int D, int NT> struct Piece {
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float acc[4] = {correction[n][k][0], correction[n][k][1], correction[n][k][0], correction[n][k][1]};
-            MmaF16(acc, Low(u0), Low(u1), High(u0), High(u1), q[n][k][0], q[n][k][1]);
-            MmaF16(acc, Low(v0), Low(v1), High(v0), High(v1), q[n][k][2], q[n][k][3]);
+            MmaF16(acc, Low(u0, a.masks), Low(u1, a.masks), High(u0, a.masks), High(u1, a.masks), q[n][k][0], q[n][k][1]);
+            MmaF16(acc, Low(v0, a.masks), Low(v1, a.masks), High(v0, a.masks), High(v1, a.masks), q[n][k][2], q[n][k][3]);
             score[half][n][0] += acc[0] * f[0][k], score[half][n][1] += acc[1] * f[0][k];
             score[half][n][2] += acc[2] * f[1][k], score[half][n][3] += acc[3] * f[1][k];
           }
@@ -323,13 +324,12 @@ template <typename T, int D, int NT> struct Piece {
             asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][r]) : "r"(Pack(p0, p1)));
           }
         // V's scales of tokens 2c, 2c + 1 and 2c + 8, 2c + 9 in this lane's group
-        const unsigned char *const values = tile + TileBytes<D>::kCodes + TileBytes<D>::kScales;
-        const unsigned short *const f = reinterpret_cast<const unsigned short *>(values + TileBytes<D>::kCodes) + (16 * half + 2 * c) * kGroups +
-                                        (g >> 1) % kGroups;
+        const unsigned values = tile + TileBytes<D>::kCodes + TileBytes<D>::kScales;
+        const unsigned f = values + TileBytes<D>::kCodes + 2 * ((16 * half + 2 * c) * kGroups + (g >> 1) % kGroups);
         __half2 scale[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          scale[r] = __halves2half2(__ushort_as_half(f[8 * r * kGroups]), __ushort_as_half(f[(8 * r + 1) * kGroups]));
+          scale[r] = __halves2half2(__ushort_as_half(LoadShared2(f + 16 * r * kGroups)), __ushort_as_half(LoadShared2(f + (16 * r + 2) * kGroups)));
 #pragma unroll
         for (int j = 0; j < kChunks; j += 2) {
           // four 8x8 matrices of 16-bit pieces: tokens 0..7 and 8..15 of chunk j, then of chunk j + 1
@@ -338,15 +338,15 @@ template <typename T, int D, int NT> struct Piece {
           const int swizzled = kChunks == 4 ? chunk ^ ((token >> 1) & 3) : chunk ^ ((token >> 2) & 1);
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(SmemAddress(values + (16 * half + token) * (D / 2) + 16 * swizzled))
+                       : "r"(values + (16 * half + token) * (D / 2) + 16 * swizzled)
                        : "memory");
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const unsigned u0 = v[2 * k], u1 = v[2 * k + 1], w0 = u0 >> 8, w1 = u1 >> 8;
-            const unsigned a0 = Scaled(Low(u0), 0x64086408u, scale[0]), a1 = Scaled(High(u0), 0x54805480u, scale[0]);
-            const unsigned a2 = Scaled(Low(u1), 0x64086408u, scale[1]), a3 = Scaled(High(u1), 0x54805480u, scale[1]);
-            const unsigned b0 = Scaled(Low(w0), 0x64086408u, scale[0]), b1 = Scaled(High(w0), 0x54805480u, scale[0]);
-            const unsigned b2 = Scaled(Low(w1), 0x64086408u, scale[1]), b3 = Scaled(High(w1), 0x54805480u, scale[1]);
+            const unsigned a0 = Scaled(Low(u0, a.masks), 0x64086408u, scale[0]), a1 = Scaled(High(u0, a.masks), 0x54805480u, scale[0]);
+            const unsigned a2 = Scaled(Low(u1, a.masks), 0x64086408u, scale[1]), a3 = Scaled(High(u1, a.masks), 0x54805480u, scale[1]);
+            const unsigned b0 = Scaled(Low(w0, a.masks), 0x64086408u, scale[0]), b1 = Scaled(High(w0, a.masks), 0x54805480u, scale[0]);
+            const unsigned b2 = Scaled(Low(w1, a.masks), 0x64086408u, scale[1]), b3 = Scaled(High(w1, a.masks), 0x54805480u, scale[1]);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               MmaF16(o[n][2 * (j + k)], a0, a1, a2, a3, p[n][0], p[n][1]);
@@ -554,7 +554,7 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
     return PADRA_INTERNAL;
   AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * 1.4426950408889634f : 1.f,
                   scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f, window,
-                  static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), bad};
+                  static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), kCodeMasks, bad};
   if (type == PADRA_ROWS_BF16)
     return c.head_dim == 64 ? LaunchColumns<__nv_bfloat16, 64>(a, sms, stream) : LaunchColumns<__nv_bfloat16, 128>(a, sms, stream);
   return c.head_dim == 64 ? LaunchColumns<__half, 64>(a, sms, stream) : LaunchColumns<__half, 128>(a, sms, stream);

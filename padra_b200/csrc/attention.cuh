@@ -12,6 +12,13 @@ constexpr float kNever = -1e30f; // the running maximum before any token
 constexpr float kTop = 8.f, kRaise = 15.f; // log2 of the largest weight after a raise / before the next
 constexpr int kMaxGrid = 512, kMaxWideGrid = 160; // CTAs that the workspace provides for, of either kernel
 
+// Two codes as FP16 numbers: nibbles 0 and 4 of a word become 1024 + n, nibbles 1 and 5 become 64 + n, one logic operation each.
+// The masks come from the kernel's arguments: as literals the compiler spends two operations (AND, OR) on every one.
+struct CodeMasks {
+  unsigned low, high, low_base, high_base;
+};
+constexpr CodeMasks kCodeMasks{0x000f000fu, 0x00f000f0u, 0x64006400u, 0x54005400u};
+
 // The unit that begins in a CTA's run and goes on in others': how many pieces there are (0: no such unit), in which slot this
 // CTA left the first one (the others are in their CTAs' slot 0), and where the output goes.
 struct Split {
@@ -30,15 +37,17 @@ struct AttentionArgs {
   int window;
   struct Split *split; // [grid]
   float *partial;      // [grid][2]: outputs [columns][head_dim], then maximum and sum [columns][2]
+  CodeMasks masks;
   int *bad;
 };
 
-__device__ __forceinline__ unsigned Low(unsigned w) { // nibbles 0 and 4 as 1024 + n
-  return (w & 0x000f000fu) | 0x64006400u;
+__device__ __forceinline__ unsigned MaskOr(unsigned w, unsigned mask, unsigned base) {
+  unsigned r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(base)); // (w & mask) | base
+  return r;
 }
-__device__ __forceinline__ unsigned High(unsigned w) { // nibbles 1 and 5 as 64 + n
-  return (w & 0x00f000f0u) | 0x54005400u;
-}
+__device__ __forceinline__ unsigned Low(unsigned w, const CodeMasks &m) { return MaskOr(w, m.low, m.low_base); }
+__device__ __forceinline__ unsigned High(unsigned w, const CodeMasks &m) { return MaskOr(w, m.high, m.high_base); }
 __device__ __forceinline__ unsigned Scaled(unsigned x, unsigned offset, __half2 scale) {
   const __half2 v = __hmul2(__hsub2(*reinterpret_cast<__half2 *>(&x), *reinterpret_cast<__half2 *>(&offset)), scale);
   return *reinterpret_cast<const unsigned *>(&v);
@@ -72,6 +81,31 @@ __device__ __forceinline__ void Store4(__nv_bfloat16 *p, float4 v) {
 }
 __device__ __forceinline__ void Store4(__half *p, float4 v) {
   *reinterpret_cast<uint2 *>(p) = make_uint2(Pack(v.x, v.y), Pack(v.z, v.w));
+}
+
+// Shared memory by 32-bit address: through pointers the compiler used 64-bit generic addresses, several operations for each access.
+__device__ __forceinline__ void StoreShared(unsigned address, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 LoadShared16(unsigned address) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 LoadShared8(unsigned address) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned LoadShared4(unsigned address) {
+  unsigned v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned short LoadShared2(unsigned address) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address) : "memory");
+  return v;
 }
 
 // a / b of numbers that are nearly always below 2^32, where the division is much cheaper
