@@ -8,7 +8,7 @@
 //     rounding of 2^-12) in the 128-byte-swizzled layout, the same for K (K-major: contraction over the head's values) and V
 //     (MN-major: contraction over tokens), so that V needs no transposition.  Values inside a block of eight lie in the order
 //     0 4 1 5 2 6 3 7 in which a code word yields pairs; Q is stored in that order and the output put back.
-//   * A thread for each half issues its MMAs: S (128 columns x 128 tokens) of each half of the block in its own tensor memory, so that one
+//   * One thread issues the MMAs: S (128 columns x 128 tokens) of each half of the block in its own tensor memory, so that one
 //     half's MMAs run under the other half's softmax.  P replaces S in tensor memory as the A operand of O += P V.
 //   * Two softmax warpgroups, one per half, one thread per column: no shuffles.  The maximum is raised lazily (by a factor of up to
 //     2^15 in FP16 weights), and only then is O rescaled.
@@ -22,9 +22,11 @@ namespace padra {
 namespace attention {
 namespace {
 
-constexpr int kTile = 128, kSub = 64, kColumns = 256; // scores and weights go by sub-tiles of 64 tokens
+constexpr int kTile = 128, kColumns = 256;
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 8, kMmaWarp = kSoftmaxWarps + kProducerWarps;
-constexpr int kWarps = kMmaWarp + 2, kThreads = kWarps * 32;
+constexpr int kWarps = kMmaWarp + 4, kThreads = kWarps * 32; // whole warpgroups, for the register split; three warps idle
+// Registers per thread: launched with 96 (640 threads), then split 2 * 120 + 2 * 88 + 64 = 5 * 96.
+constexpr int kSoftmaxRegisters = 120, kProducerRegisters = 88, kMmaRegisters = 64;
 constexpr int kStages = 2;
 
 // place / group and its remainder inside a unit: `reciprocal` = ceil(2^32 / group) gives the quotient exactly while
@@ -68,35 +70,49 @@ __device__ __forceinline__ Unit UnitOf(const AttentionArgs &a, const Rows &r, in
   return u;
 }
 
-// A CTA's run, piece by piece; every role walks it by itself.
+// What a unit takes beyond its tiles (queries in, output out, the pipeline's filling), in tiles: the list of work counts it, or CTAs with
+// many short units would take several times as long as those with a part of a long one.
+constexpr int kSetup = 4;
+
+// A CTA's run, piece by piece; every role walks it by itself.  A unit is kSetup + tiles long in the list.
 struct Walk {
   long long at, end;
-  int s, block, head, skip; // the piece begins `skip` tiles into its unit
+  int s, block, head;
+  int from, span;  // the piece's place in its unit, in the list's measure
+  int skip, count; // and in tiles: the piece begins `skip` tiles into its unit
   Rows rows;
   Unit unit;
-  int count;
-  __device__ __noinline__ void Begin(const AttentionArgs &a, long long from, long long to, int sequence, int first_block, long long offset) {
-    at = from, end = to, s = sequence, block = first_block;
+  __device__ __forceinline__ void Place(int x) {
+    from = x, span = static_cast<int>(min(static_cast<long long>(kSetup + unit.tiles - x), end - at));
+    skip = max(0, x - kSetup), count = max(0, x + span - kSetup) - skip;
+  }
+  __device__ __forceinline__ void Begin(const AttentionArgs &a, long long first, long long last, int sequence, int first_block, long long offset) {
+    at = first, end = last, s = sequence, block = first_block;
     rows = RowsOf(a, s), unit = UnitOf(a, rows, block);
-    head = static_cast<int>(Quotient(offset, unit.tiles)), skip = static_cast<int>(offset - static_cast<long long>(head) * unit.tiles);
-    count = static_cast<int>(min(static_cast<long long>(unit.tiles - skip), end - at));
+    const int length = kSetup + unit.tiles;
+    head = static_cast<int>(Quotient(offset, length));
+    Place(static_cast<int>(offset - static_cast<long long>(head) * length));
+    if (!count)
+      Next(a);
   }
   __device__ __forceinline__ bool More() const { return at < end; }
-  __device__ __noinline__ void Next(const AttentionArgs &a) {
-    at += count, skip = 0;
-    if (at >= end)
-      return;
-    if (++head == a.cache.kv_heads) {
-      head = 0;
-      if (++block == rows.blocks) {
-        block = 0;
-        do
-          rows = RowsOf(a, ++s);
-        while (!rows.blocks);
+  __device__ __forceinline__ void Next(const AttentionArgs &a) { // the next piece with tiles
+    do {
+      at += span;
+      if (at >= end)
+        return;
+      if (++head == a.cache.kv_heads) {
+        head = 0;
+        if (++block == rows.blocks) {
+          block = 0;
+          do
+            rows = RowsOf(a, ++s);
+          while (!rows.blocks);
+        }
+        unit = UnitOf(a, rows, block);
       }
-      unit = UnitOf(a, rows, block);
-    }
-    count = static_cast<int>(min(static_cast<long long>(unit.tiles), end - at));
+      Place(0);
+    } while (!count);
   }
   __device__ __forceinline__ bool Paired() const { return unit.columns <= 128; }
 };
@@ -106,7 +122,7 @@ template <int D> struct Smem {
   alignas(1024) unsigned char q[2][kHalves][128 * 128]; // rows of 64 values (128 bytes), 16-byte pieces swizzled by row
   alignas(1024) unsigned char k[kStages][kHalves][kTile * 128];
   alignas(1024) unsigned char v[kStages][kHalves][kTile * 128];
-  alignas(8) unsigned long long q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2][2], p_full[2][2], o_full[2], o_last[2]; // [half][sub-tile]; O after every sub-tile, after a piece's last
+  alignas(8) unsigned long long q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
   unsigned long long q_empty;
   unsigned long long shared_ready, shared_done; // the second half's maximum and sum are there / have been used
   struct {
@@ -118,25 +134,24 @@ template <int D> struct Smem {
   int item_begin[kThreads];
   long long scan[kWarps], start_offset;
   int start_sequence, start_block;
-  Walk walk[kMmaWarp + 2]; // every working warp's place in the run: in registers it crowded out what the loops need
+  Walk walk[kMmaWarp + 1]; // every working warp's place in the run: in registers it crowded out what the loops need
   unsigned tmem;
   int abort;
 };
 
-// Bounded wait (see BarrierWait).  Code size is what this kernel's three roles compete for: with every wait written out they did not fit the
-// instruction cache together and fetched their loops anew for every tile.  So a wait is one poll in place (which the hardware may
-// suspend) and a call for the rest.
-__device__ __forceinline__ bool Passed(unsigned address, unsigned parity) {
-  unsigned done;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-               : "=r"(done)
-               : "r"(address), "r"(parity), "r"(2000u)
-               : "memory");
-  return done != 0;
-}
-__device__ __noinline__ bool WaitOn(unsigned address, unsigned parity, const volatile int *abort) {
+// Bounded wait (see BarrierWait) that lets the hardware suspend the thread for up to two microseconds at a time: seventeen warps wait
+// here most of the time, and plain polling took issue slots from the ones at work.
+__device__ __forceinline__ bool SuspendedWait(unsigned long long *bar, unsigned parity, const volatile int *abort) {
+  const unsigned address = SmemAddress(bar);
   unsigned long long started = 0;
-  while (!Passed(address, parity)) {
+  for (;;) {
+    unsigned done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(address), "r"(parity), "r"(2000u)
+                 : "memory");
+    if (done)
+      return true;
     if (*abort)
       return false;
     unsigned long long now;
@@ -146,11 +161,6 @@ __device__ __noinline__ bool WaitOn(unsigned address, unsigned parity, const vol
     else if (now - started > kWaitLimitNs)
       return false;
   }
-  return true;
-}
-__device__ __forceinline__ bool SuspendedWait(unsigned long long *bar, unsigned parity, const volatile int *abort) {
-  const unsigned address = SmemAddress(bar);
-  return Passed(address, parity) || WaitOn(address, parity, abort);
 }
 // One lane waits for its warp: true for all lanes or for none.
 __device__ __forceinline__ bool WarpWait(unsigned long long *bar, unsigned parity, const volatile int *abort) {
@@ -192,33 +202,44 @@ __device__ __forceinline__ void TmemStore16(unsigned taddr, const unsigned (&v)[
                "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                : "memory");
 }
-// Columns of the thread's lane, in pairs for the packed FP32 operations.  One statement with the wait: nothing that uses a value can
-// move before it, and the pairs are the registers that the load fills.
-using Pair = unsigned long long;
-__device__ __forceinline__ void TmemLoadPairs(unsigned taddr, Pair (&v)[8]) {
-  asm volatile("{\n\t.reg .b32 r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15;\n\t"
-               "tcgen05.ld.sync.aligned.32x32b.x16.b32 {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15}, [%8];\n\t"
-               "tcgen05.wait::ld.sync.aligned;\n\t"
-               "mov.b64 %0, {r0, r1}; mov.b64 %1, {r2, r3}; mov.b64 %2, {r4, r5}; mov.b64 %3, {r6, r7};\n\t"
-               "mov.b64 %4, {r8, r9}; mov.b64 %5, {r10, r11}; mov.b64 %6, {r12, r13}; mov.b64 %7, {r14, r15};\n\t"
-               "}"
-               : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]), "=l"(v[7])
-               : "r"(taddr)
+__device__ __forceinline__ void TmemStore32(unsigned taddr, const unsigned (&v)[32]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+               "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+               "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+               "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
                : "memory");
 }
-__device__ __forceinline__ void TmemLoadPairs(unsigned taddr, Pair (&v)[16]) {
-  asm volatile("{\n\t.reg .b32 r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31;\n\t"
-               "tcgen05.ld.sync.aligned.32x32b.x32.b32 {r0, r1, r2, r3, r4, r5, r6, r7, r8, r9, r10, r11, r12, r13, r14, r15, r16, r17, r18, r19, r20, r21, r22, r23, r24, r25, r26, r27, r28, r29, r30, r31}, [%16];\n\t"
-               "tcgen05.wait::ld.sync.aligned;\n\t"
-               "mov.b64 %0, {r0, r1}; mov.b64 %1, {r2, r3}; mov.b64 %2, {r4, r5}; mov.b64 %3, {r6, r7};\n\t"
-               "mov.b64 %4, {r8, r9}; mov.b64 %5, {r10, r11}; mov.b64 %6, {r12, r13}; mov.b64 %7, {r14, r15};\n\t"
-               "mov.b64 %8, {r16, r17}; mov.b64 %9, {r18, r19}; mov.b64 %10, {r20, r21}; mov.b64 %11, {r22, r23};\n\t"
-               "mov.b64 %12, {r24, r25}; mov.b64 %13, {r26, r27}; mov.b64 %14, {r28, r29}; mov.b64 %15, {r30, r31};\n\t"
-               "}"
-               : "=l"(v[0]), "=l"(v[1]), "=l"(v[2]), "=l"(v[3]), "=l"(v[4]), "=l"(v[5]), "=l"(v[6]), "=l"(v[7]),
-                 "=l"(v[8]), "=l"(v[9]), "=l"(v[10]), "=l"(v[11]), "=l"(v[12]), "=l"(v[13]), "=l"(v[14]), "=l"(v[15])
+// Columns of the thread's lane.
+__device__ __forceinline__ void TmemLoad16(unsigned taddr, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                 "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
                : "r"(taddr)
                : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    asm volatile("" : "+f"(v[i])); // no use of a value moves up across the wait
+}
+__device__ __forceinline__ void TmemLoad64(unsigned taddr, float (&v)[64]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]),
+                 "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]),
+                 "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]),
+                 "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+                 "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]), "=f"(v[38]), "=f"(v[39]),
+                 "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]), "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]),
+                 "=f"(v[48]), "=f"(v[49]), "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+                 "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]), "=f"(v[62]), "=f"(v[63])
+               : "r"(taddr)
+               : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i)
+    asm volatile("" : "+f"(v[i])); // no use of a value moves up across the wait
 }
 __device__ __forceinline__ void TmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -231,8 +252,8 @@ __device__ __forceinline__ unsigned PieceOffset(int row, int piece) {
 template <int D> struct Producer {
   static constexpr int kGroups = D / kKvGroup, kChunks = D / 32; // 16-byte chunks of a token's codes
   static constexpr int kTokens = 16 * kChunks / 32;              // tokens per lane: its warp's 16 tokens, one chunk each
-  uint4 codes[kTokens];
-  uint2 scales[kTokens]; // of the token's groups (head size 64: in .x)
+  uint4 k[kTokens], v[kTokens];
+  uint2 k_scale[kTokens], v_scale[kTokens]; // the groups' scales (head size 64: in .x)
 
   // Lanes of a quarter warp (whose stores go out together) take rows whose swizzle leaves no bank twice: rows t and t + 4 with
   // four chunks, rows {0, 1, 4, 5} or {2, 3, 6, 7} with two.
@@ -242,61 +263,53 @@ template <int D> struct Producer {
     else
       return (lane >> 4) * 8 + ((lane >> 3) & 1) * 2 + ((lane >> 1) & 1) + ((lane >> 2) & 1) * 4;
   }
-  // Codes and scales of this warp's 16 tokens, of which `there` exist (their codes begin at `codes_from`, their scales at `scales_from`): lanes
-  // beyond them read the last one that exists and take scales of zero.
-  __device__ __forceinline__ void Load(const unsigned char *codes_from, const unsigned char *scales_from, int there) {
-    const int lane = threadIdx.x & 31;
+  // Codes and scales of this warp's 16 tokens from token t on; zeros (scale 0) for tokens at and beyond `context` or without a page.
+  __device__ __forceinline__ void Load(const AttentionArgs &a, int page, int head, int t, int context) {
+    const int lane = threadIdx.x & 31, chunk = lane % kChunks;
+    const unsigned char *const block = a.cache.block(max(page, 0), head);
+    const int slot = t & (a.cache.page_size - 1), code_bytes = a.cache.code_bytes(), both = code_bytes + a.cache.scale_bytes();
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
-      const int token = TokenOf(lane, i), row = max(0, min(token, there - 1));
-      codes[i] = __ldg(reinterpret_cast<const uint4 *>(codes_from + row * (D / 2) + 16 * (lane % kChunks)));
-      if constexpr (kGroups == 4)
-        scales[i] = __ldg(reinterpret_cast<const uint2 *>(scales_from + row * (D / 16)));
-      else
-        scales[i] = make_uint2(__ldg(reinterpret_cast<const unsigned *>(scales_from + row * (D / 16))), 0);
-      if (token >= there)
-        scales[i] = make_uint2(0, 0);
+      const int token = TokenOf(lane, i);
+      k[i] = v[i] = make_uint4(0, 0, 0, 0), k_scale[i] = v_scale[i] = make_uint2(0, 0);
+      if (page >= 0 && t + token < context) {
+        const unsigned char *const codes = block + (slot + token) * (D / 2) + 16 * chunk, *const scales = block + code_bytes + (slot + token) * (D / 16);
+        k[i] = __ldg(reinterpret_cast<const uint4 *>(codes)), v[i] = __ldg(reinterpret_cast<const uint4 *>(codes + both));
+        if constexpr (kGroups == 4) {
+          k_scale[i] = __ldg(reinterpret_cast<const uint2 *>(scales)), v_scale[i] = __ldg(reinterpret_cast<const uint2 *>(scales + both));
+        } else {
+          k_scale[i].x = __ldg(reinterpret_cast<const unsigned *>(scales)), v_scale[i].x = __ldg(reinterpret_cast<const unsigned *>(scales + both));
+        }
+      }
     }
   }
-  // Byte offset of the first word's piece of (row, chunk) in a tile: word c * groups + g of a row holds piece 4 g + c of eight values.
-  static __device__ __forceinline__ unsigned OffsetOf(int row, int chunk) { return PieceOffset(row, 4 * chunk / kGroups); }
-  // Word w of the chunk lies 4 (w % groups) + w / groups pieces on; pieces 0 .. 7 of a half change places with the row (XOR), so
-  // neighbours are found by XOR too: bit 2 of the piece is bit 6 of the offset.
-  static __device__ __forceinline__ void Store(unsigned tile, unsigned offset, const uint4 &codes, const uint2 &scales, const CodeMasks &masks) {
+  static __device__ __forceinline__ void Store(unsigned tile, int row, int chunk, const uint4 &codes, const uint2 &scales, const CodeMasks &masks) {
     const unsigned word[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const int g = w % kGroups, c = w / kGroups;
-      const unsigned pair = g & 2 ? scales.y : scales.x;
+      const int place = 4 * chunk + w, piece = 4 * (place % kGroups) + place / kGroups; // word c * groups + g holds piece 4 g + c
+      const unsigned pair = (w % kGroups) & 2 ? scales.y : scales.x;                    // place % groups == w % groups
       const __half2 both = *reinterpret_cast<const __half2 *>(&pair), scale = w & 1 ? __high2half2(both) : __low2half2(both);
       const unsigned u = word[w], x = u >> 8;
-      StoreShared(tile + (offset ^ ((g & 1) << 6 | c << 4)) + (g >> 1) * (128 * 128),
-                  make_uint4(Scaled(Low(u, masks), 0x64086408u, scale), Scaled(High(u, masks), 0x54805480u, scale),
-                             Scaled(Low(x, masks), 0x64086408u, scale), Scaled(High(x, masks), 0x54805480u, scale)));
+      StoreShared(tile + PieceOffset(row, piece), make_uint4(Scaled(Low(u, masks), 0x64086408u, scale), Scaled(High(u, masks), 0x54805480u, scale),
+                                                             Scaled(Low(x, masks), 0x64086408u, scale), Scaled(High(x, masks), 0x54805480u, scale)));
     }
   }
 };
 
 // ---- softmax ----
-__device__ __forceinline__ Pair MakePair(float x, float y) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
-  return p;
-}
-__device__ __forceinline__ void SplitPair(Pair p, float *x, float *y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(*x), "=f"(*y) : "l"(p)); }
-__device__ __forceinline__ Pair Fma2(Pair x, Pair y, Pair z) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+__device__ __forceinline__ float2 Fma2(float2 x, float2 y, float2 z) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y), "f"(z.x), "f"(z.y));
   return r;
 }
-__device__ __forceinline__ Pair Mul2(Pair x, Pair y) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-  return r;
-}
-__device__ __forceinline__ Pair Add2(Pair x, Pair y) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+__device__ __forceinline__ float2 Add2(float2 x, float2 y) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x.x), "f"(x.y), "f"(y.x), "f"(y.y));
   return r;
 }
 __device__ __forceinline__ float Max3(float x, float y, float z) {
@@ -372,97 +385,6 @@ __device__ __forceinline__ void StageQueries(const AttentionArgs &a, const Rows 
   }
 }
 
-// The MMAs of one half, issued by one thread: S of a tile's two sub-tiles, then O of a sub-tile and S of the same sub-tile of the next tile.  So S is
-// ready a sub-tile before its softmax begins, and softmax and tensor cores do not wait for each other in turn.  In blocks with
-// columns for both halves every tile is the half's, otherwise every other one.  Each half has a thread of its own, on another scheduler:
-// between the many warps an MMA's ten instructions take longer to come by than its 64 cycles on the tensor cores.  Half and sub-tile
-// are compile-time and tensor memory begins at column 0 (the CTA has all of it): with addresses in registers an MMA took up to a
-// hundred instructions.
-template <int D, int Half, int Sub> __device__ __forceinline__ void IssueScores(unsigned q_low, unsigned k_low) {
-#pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
-    const unsigned offset = ((s >> 2) * (128 * 128) + (s & 3) * 32) >> 4;
-    MmaStepSS(128 * Half + kSub * Sub, q_low + offset, k_low + offset + ((Sub * kSub * 128) >> 4), InstructionDescriptor(kSub), s > 0);
-  }
-}
-template <int D, int Half, int Sub> __device__ __forceinline__ void IssueOutput(unsigned v_low, bool accumulate) {
-#pragma unroll
-  for (int s = 0; s < kSub / 16; ++s)
-    MmaStepTS(256 + 128 * Half, 128 * Half + kSub * Sub + 8 * s, v_low + (((Sub * kSub + 16 * s) * 128) >> 4),
-              InstructionDescriptor(D) | kSecondOperandRowMajor, accumulate || s > 0);
-}
-template <int D, int Half> __device__ __forceinline__ bool IssueMmas(const AttentionArgs &a, Smem<D> &sm, Walk &walk) {
-  const volatile int *const abort = &sm.abort;
-  unsigned tiles = 0, jobs = 0, pieces = 0, staged = 0; // so far: tiles, this half's jobs, pieces, pieces with queries of its own
-  bool alive = true;
-  for (; alive && walk.More(); walk.Next(a), ++pieces) {
-    const bool paired = walk.Paired();
-    const int count = walk.count, step = paired ? 2 : 1, first = paired ? Half : 0;
-    auto wait = [&](unsigned long long *full, int tile) { return SuspendedWait(full + ((tiles + tile) & (kStages - 1)), ((tiles + tile) / kStages) & 1, abort); };
-    // A tile that is the other half's is released here too, once it is there (an arrival must not count for an earlier tile).
-    auto pass = [&](unsigned long long *full, unsigned long long *empty, int tile) {
-      if (tile < 0 || tile >= count || !paired)
-        return true;
-      const bool there = wait(full, tile);
-      BarrierArrive(empty + ((tiles + tile) & (kStages - 1)));
-      return there;
-    };
-    auto q_low = [&] { return DescriptorLow(SmemAddress(sm.q[Half && !paired][0]), 16); };
-    auto stage_of = [&](int tile) { return (tiles + tile) & (kStages - 1); };
-    auto first_scores = [&](int tile) {
-      if (!pass(sm.k_full, sm.k_empty, tile - 1) || !wait(sm.k_full, tile))
-        return false;
-      AfterSync();
-      IssueScores<D, Half, 0>(q_low(), DescriptorLow(SmemAddress(sm.k[stage_of(tile)][0]), 16));
-      MmaCommit(&sm.s_full[Half][0]);
-      return true;
-    };
-    auto second_scores = [&](int tile) {
-      IssueScores<D, Half, 1>(q_low(), DescriptorLow(SmemAddress(sm.k[stage_of(tile)][0]), 16));
-      MmaCommit(&sm.s_full[Half][1]);
-      MmaCommit(&sm.k_empty[stage_of(tile)]);
-      if (tile + step >= count)
-        MmaCommit(&sm.q_empty);
-    };
-    alive = Half && !paired ? SuspendedWait(&sm.q_full[1], staged++ & 1, abort) : SuspendedWait(&sm.q_full[0], pieces & 1, abort);
-    if (!alive)
-      break;
-    if (first >= count) // a single tile, the other half's
-      BarrierArrive(&sm.q_empty);
-    int tile = first - step; // the first turn of the loop has scores only
-    for (; alive && tile < count; tile += step) {
-      const int next = tile + step;
-      const unsigned v_low = DescriptorLow(SmemAddress(sm.v[stage_of(tile)][0]), 128 * 128);
-      if (tile >= first) {
-        if (!(alive = pass(sm.v_full, sm.v_empty, tile - 1) && wait(sm.v_full, tile) && SuspendedWait(&sm.p_full[Half][0], jobs & 1, abort)))
-          break;
-        AfterSync();
-        IssueOutput<D, Half, 0>(v_low, tile > first);
-        MmaCommit(&sm.o_full[Half]);
-      }
-      if (next < count && !(alive = first_scores(next)))
-        break;
-      if (tile >= first) {
-        if (!(alive = SuspendedWait(&sm.p_full[Half][1], jobs & 1, abort)))
-          break;
-        AfterSync();
-        IssueOutput<D, Half, 1>(v_low, true);
-        MmaCommit(&sm.o_full[Half]);
-        MmaCommit(&sm.v_empty[stage_of(tile)]);
-        ++jobs;
-      }
-      if (next < count)
-        second_scores(next);
-      else if (tile >= first)
-        MmaCommit(&sm.o_last[Half]);
-    }
-    if (alive) // what follows this half's last tile
-      alive = pass(sm.k_full, sm.k_empty, tile - 1) && pass(sm.v_full, sm.v_empty, tile - 1);
-    tiles += count;
-  }
-  return alive;
-}
-
 template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) WideAttentionKernel(const __grid_constant__ AttentionArgs a) {
   using S = Smem<D>;
   extern __shared__ __align__(16) unsigned char raw_smem[];
@@ -494,7 +416,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
               high = middle - 1;
           }
           item_sequence = s0 + low, item_block = i - sm.item_begin[low];
-          cost_mine = static_cast<long long>(UnitOf(a, RowsOf(a, item_sequence), item_block).tiles) * a.cache.kv_heads;
+          cost_mine = static_cast<long long>(kSetup + UnitOf(a, RowsOf(a, item_sequence), item_block).tiles) * a.cache.kv_heads;
         }
         long long part;
         at_mine = total + BlockPrefix<kWarps>(cost_mine, sm.scan, &part);
@@ -506,20 +428,19 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     }
   };
   scan(-1);
-  const long long share = max(2ll, Quotient(total + gridDim.x - 1, gridDim.x)), begin = blockIdx.x * share, end = min(total, begin + share);
+  const long long share = max(2ll + kSetup, Quotient(total + gridDim.x - 1, gridDim.x)), begin = blockIdx.x * share, end = min(total, begin + share);
   if (tid == 0) {
     a.split[blockIdx.x].pieces = 0;
     sm.abort = 0;
     for (int i = 0; i < 2; ++i) {
-      BarrierInit(&sm.q_full[i], kProducerWarps / 2), BarrierInit(&sm.o_full[i], 1), BarrierInit(&sm.o_last[i], 1);
-      for (int sub = 0; sub < 2; ++sub)
-        BarrierInit(&sm.s_full[i][sub], 1), BarrierInit(&sm.p_full[i][sub], kSoftmaxWarps / 2);
+      BarrierInit(&sm.q_full[i], kProducerWarps / 2), BarrierInit(&sm.s_full[i], 1);
+      BarrierInit(&sm.p_full[i], kSoftmaxWarps / 2), BarrierInit(&sm.o_full[i], 1);
     }
     for (int i = 0; i < kStages; ++i) {
       BarrierInit(&sm.k_full[i], kProducerWarps), BarrierInit(&sm.v_full[i], kProducerWarps);
-      BarrierInit(&sm.k_empty[i], 2), BarrierInit(&sm.v_empty[i], 2); // both halves let go of a tile
+      BarrierInit(&sm.k_empty[i], 1), BarrierInit(&sm.v_empty[i], 1);
     }
-    BarrierInit(&sm.q_empty, 2);
+    BarrierInit(&sm.q_empty, 1);
     BarrierInit(&sm.shared_ready, kSoftmaxWarps / 2), BarrierInit(&sm.shared_done, kSoftmaxWarps / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -538,10 +459,10 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
   BeforeSync();
   __syncthreads();
   AfterSync();
-  constexpr unsigned tmem = 0; // all 512 columns are this CTA's
+  const unsigned tmem = sm.tmem;
   const volatile int *const abort = &sm.abort;
-  Walk &walk = sm.walk[min(warp, kMmaWarp + 1)];
-  if (lane == 0 && warp <= kMmaWarp + 1)
+  Walk &walk = sm.walk[min(warp, kMmaWarp)];
+  if (lane == 0 && warp <= kMmaWarp)
     walk.Begin(a, begin, end, sm.start_sequence, sm.start_block, sm.start_offset);
   __syncwarp();
   auto next_piece = [&]() { // by the whole warp
@@ -550,44 +471,24 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       walk.Next(a);
     __syncwarp();
   };
-  bool alive = sm.tmem == 0;
+  bool alive = true;
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
     // =============================== producers ===============================
     using P = Producer<D>;
-    const int mine = 16 * (warp - kSoftmaxWarps); // this warp's tokens of a tile
-    unsigned offset[P::kTokens];
-#pragma unroll
-    for (int j = 0; j < P::kTokens; ++j)
-      offset[j] = P::OffsetOf(mine + P::TokenOf(lane, j), lane % P::kChunks);
-    int tile = 0; // of the piece: the tile that is loaded next
-    const unsigned char *codes_from = a.cache.pool, *scales_from = a.cache.pool; // K's codes and scales of the warp's tokens in it
-    int there = 0;                                                             // how many of them the columns may see
-    const int v_behind = a.cache.code_bytes() + a.cache.scale_bytes();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
+    const int mine = 16 * (warp - kSoftmaxWarps), chunk = lane % P::kChunks; // this warp's tokens of a tile
+    int tile = 0, page = -1; // of the piece: the tile that is loaded next, and the page of the warp's tokens in it
+    P data;
     auto find = [&]() {
-      there = 0;
+      page = -1;
       if (walk.More()) {
-        const int t = (walk.unit.first + walk.skip + tile) * kTile + mine, context = walk.rows.context;
+        const int t = (walk.unit.first + walk.skip + tile) * kTile + mine;
         // first token that some column of the unit sees
-        const int low = a.window ? max(0, context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
-        if (t < context && t + 16 > low) {
-          const int page = PageOf(a.seq, a.cache, walk.s, t, a.bad), slot = t & (a.cache.page_size - 1);
-          if (page >= 0) {
-            const unsigned char *const block = a.cache.block(page, walk.head);
-            codes_from = block + slot * (D / 2), scales_from = block + a.cache.code_bytes() + slot * (D / 16);
-            there = min(16, context - t);
-          }
-        }
+        const int low = a.window ? max(0, walk.rows.context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
+        if (t < walk.rows.context && t + 16 > low)
+          page = PageOf(a.seq, a.cache, walk.s, t, a.bad);
       }
-    };
-    auto advance = [&]() {
-      if (++tile == walk.count)
-        next_piece(), tile = 0;
-      find();
-    };
-    auto load = [&](P &to, bool is_v) {
-      const int behind = is_v ? v_behind : 0;
-      to.Load(codes_from + behind, scales_from + behind, there);
     };
     // A piece's queries come before its first tile: this warp's 32 columns, once the MMAs of the piece before are done with Q.
     unsigned pieces = 0;
@@ -604,41 +505,107 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       }
       ++pieces;
     };
-    // K and V of a tile are two steps of the same code; what is stored next has been loaded two steps before.
-    P front, back;
-    find();
-    const int steps = 2 * static_cast<int>(end - begin);
-#pragma unroll 1
-    for (int n = -2; n < steps && alive; ++n) {
-      const bool is_v = n & 1;
-      if (n >= 0) {
-        const int stage = (n >> 1) & (kStages - 1);
-        alive = WarpWait(is_v ? &sm.v_empty[stage] : &sm.k_empty[stage], ((n / (2 * kStages)) & 1) ^ 1, abort);
-        if (!alive)
-          break;
-        const unsigned to = SmemAddress(sm.k[0][0]) + (is_v ? kStages + stage : stage) * static_cast<unsigned>(sizeof(sm.k[0])); // V lies behind K
-#pragma unroll
-        for (int j = 0; j < P::kTokens; ++j)
-          P::Store(to, offset[j], front.codes[j], front.scales[j], a.masks);
-        FenceToTensorCores();
-        __syncwarp();
-        if (lane == 0)
-          BarrierArrive(is_v ? &sm.v_full[stage] : &sm.k_full[stage]);
+    auto load = [&]() { // that tile's codes, then the page of the one after it
+      if (walk.More()) {
+        data.Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, walk.rows.context);
+        if (++tile == walk.count)
+          next_piece(), tile = 0;
+        find();
       }
-      front = back;
-      if (n + 2 < steps) {
-        load(back, is_v); // the same of the next tile
-        if (is_v) {
-          if (tile == 0) // that tile begins a piece
-            stage_queries();
-          advance();
-        }
+    };
+    bool have = walk.More(); // a tile has been loaded and not been stored
+    if (have) {
+      find();
+      stage_queries();
+      load();
+    }
+    for (unsigned n = 0; have && alive; ++n) {
+      const int stage = n & (kStages - 1);
+      const unsigned free_parity = ((n / kStages) & 1) ^ 1;
+      alive = WarpWait(&sm.k_empty[stage], free_parity, abort);
+      if (!alive)
+        break;
+#pragma unroll
+      for (int j = 0; j < P::kTokens; ++j)
+        P::Store(SmemAddress(sm.k[stage][0]), mine + P::TokenOf(lane, j), chunk, data.k[j], data.k_scale[j], a.masks);
+      FenceToTensorCores();
+      __syncwarp();
+      if (lane == 0)
+        BarrierArrive(&sm.k_full[stage]);
+      alive = WarpWait(&sm.v_empty[stage], free_parity, abort);
+      if (!alive)
+        break;
+#pragma unroll
+      for (int j = 0; j < P::kTokens; ++j)
+        P::Store(SmemAddress(sm.v[stage][0]), mine + P::TokenOf(lane, j), chunk, data.v[j], data.v_scale[j], a.masks);
+      FenceToTensorCores();
+      __syncwarp();
+      if (lane == 0)
+        BarrierArrive(&sm.v_full[stage]);
+      have = walk.More();
+      if (have) {
+        if (tile == 0) // the next tile begins a piece
+          stage_queries();
+        load(); // arrives while the MMAs free the next stage
       }
     }
   } else if (warp >= kMmaWarp) {
     // =============================== MMA issue ===============================
-    if (lane == 0 && warp <= kMmaWarp + 1) {
-      alive = alive && (warp == kMmaWarp ? IssueMmas<D, 0>(a, sm, walk) : IssueMmas<D, 1>(a, sm, walk));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegisters));
+    // Job i of a piece: half i & 1 with tile i / 2, or with tile i where both halves work on the same columns.
+    if (warp == kMmaWarp && lane == 0) {
+      const unsigned s_desc = InstructionDescriptor(kTile), o_desc = InstructionDescriptor(D) | kSecondOperandRowMajor;
+      unsigned tiles = 0, jobs_of[2] = {0, 0}, pieces_of[2] = {0, 0}; // all so far: tiles, jobs and staged Q tiles of the halves
+      for (; alive && walk.More(); walk.Next(a)) {
+        const bool paired = walk.Paired();
+        const int jobs = paired ? walk.count : 2 * walk.count;
+        auto scores = [&](int i) { // S of job i
+          const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
+          if (paired || half == 0)
+            if (!(alive = SuspendedWait(&sm.k_full[stage], ((tiles + tile) / kStages) & 1, abort)))
+              return;
+          AfterSync();
+          const unsigned q_low = DescriptorLow(SmemAddress(sm.q[paired ? 0 : half][0]), 16), k_low = DescriptorLow(SmemAddress(sm.k[stage][0]), 16);
+#pragma unroll
+          for (int step = 0; step < D / 16; ++step) {
+            const unsigned offset = ((step >> 2) * (128 * 128) + (step & 3) * 32) >> 4;
+            MmaStepSS(tmem + 128 * half, q_low + offset, k_low + offset, s_desc, step > 0);
+          }
+          MmaCommit(&sm.s_full[half]);
+          if (paired || half == 1)
+            MmaCommit(&sm.k_empty[stage]);
+          if (i == jobs - 1)
+            MmaCommit(&sm.q_empty);
+        };
+        // Q of this piece: the second half's tile is staged only where it has columns of its own
+        alive = SuspendedWait(&sm.q_full[0], pieces_of[0]++ & 1, abort);
+        if (alive)
+          scores(0);
+        if (alive && !paired)
+          alive = SuspendedWait(&sm.q_full[1], pieces_of[1]++ & 1, abort);
+        if (alive && jobs > 1)
+          scores(1);
+        for (int i = 0; i < jobs && alive; ++i) {
+          const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
+          if (paired || half == 0)
+            if (!(alive = SuspendedWait(&sm.v_full[stage], ((tiles + tile) / kStages) & 1, abort)))
+              break;
+          if (!(alive = SuspendedWait(&sm.p_full[half], jobs_of[half]++ & 1, abort)))
+            break;
+          AfterSync();
+          const unsigned v_low = DescriptorLow(SmemAddress(sm.v[stage][0]), 128 * 128);
+#pragma unroll
+          for (int step = 0; step < kTile / 16; ++step)
+            MmaStepTS(tmem + 256 + 128 * half, tmem + 128 * half + 8 * step, v_low + step * (2048 >> 4), o_desc, i > 1 || step > 0);
+          if (paired || half == 1)
+            MmaCommit(&sm.v_empty[stage]);
+          if (i + 2 >= jobs)
+            MmaCommit(&sm.o_full[half]);
+          else
+            scores(i + 2);
+        }
+        tiles += walk.count;
+      }
       if (!alive) {
         sm.abort = 1;
         Raise(a.bad);
@@ -647,116 +614,101 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     __syncwarp();
   } else {
     // =============================== softmax ===============================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
     const int half = warp / 4, row = tid & 127; // the thread's column of its half, and its lane in tensor memory
     const unsigned lanes = static_cast<unsigned>((warp & 3) * 32) << 16, s_address = tmem + lanes + 128 * half, o_address = tmem + lanes + 256 + 128 * half;
-    // phases gone by: this half's tiles, pieces with queries of either half, O after either half's sub-tiles, joins
-    unsigned jobs = 0, staged_first = 0, staged_second = 0, outputs = 0, finished = 0, other_finished = 0, shared = 0, pieces = 0;
+    unsigned jobs = 0, staged[2] = {0, 0}, finished[2] = {0, 0}, shared = 0, pieces = 0; // phases gone by: S, Q, outputs of the halves, joins
     for (; alive && walk.More(); next_piece(), ++pieces) {
       const bool paired = walk.Paired();
       const int own = paired ? row : 128 * half + row; // column of the block
       const bool there = own < walk.unit.columns;
       // the block's columns are staged by the producers, those that both halves work on once
       if (paired || !half) {
-        alive = WarpWait(&sm.q_full[0], staged_first & 1, abort);
+        alive = WarpWait(&sm.q_full[0], staged[0]++ & 1, abort);
+        staged[1] += !paired;
       } else {
-        alive = WarpWait(&sm.q_full[1], staged_second & 1, abort);
+        ++staged[0];
+        alive = WarpWait(&sm.q_full[1], staged[1]++ & 1, abort);
       }
-      ++staged_first, staged_second += !paired;
       if (!alive)
         break;
       const float factor = sm.column[pieces & 1][own].factor;
       const int last = sm.column[pieces & 1][own].last, first = a.window ? max(0, last - a.window + 1) : 0;
       float top = kNever, total = 0;
       const int least = __reduce_min_sync(0xffffffffu, there ? last : 0x7fffffff), latest = __reduce_max_sync(0xffffffffu, there ? first : 0);
-      const int first_tile = walk.unit.first + walk.skip, count = walk.count;
-      const int begin_tile = paired ? half : 0, end_sub = 2 * count;
-      // sub-tiles of this half: both of every tile, or of every other one
-      for (int i = 2 * begin_tile; i < end_sub; i += i & 1 && paired ? 3 : 1) {
-        const int sub = i & 1, t0 = first_tile * kTile + i * kSub;
-        const unsigned score_address = s_address + kSub * sub;
-        alive = WarpWait(&sm.s_full[half][sub], jobs & 1, abort);
+      const int first_tile = walk.unit.first + walk.skip;
+      const int step = paired ? 2 : 1, begin_tile = paired ? half : 0;
+      for (int i = begin_tile; i < walk.count; i += step, ++jobs) {
+        const int t0 = (first_tile + i) * kTile;
+        alive = WarpWait(&sm.s_full[half], jobs & 1, abort);
         if (!alive)
           break;
         AfterSync();
-        if (t0 + kSub - 1 > least || t0 < latest) { // some column does not see all of the sub-tile: masked in place
+        if (t0 + kTile - 1 > least || t0 < latest) { // some column does not see all of the tile: masked in place
 #pragma unroll 1
-          for (int piece = 0; piece < kSub / 16; ++piece) {
-            Pair x[8];
+          for (int piece = 0; piece < kTile / 16; ++piece) {
+            float x[16];
             unsigned y[16];
-            TmemLoadPairs(score_address + 16 * piece, x);
+            TmemLoad16(s_address + 16 * piece, x);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               const int t = t0 + 16 * piece + j;
-              y[j] = t < first || t > last ? 0xff800000u : static_cast<unsigned>(x[j / 2] >> 32 * (j & 1));
+              y[j] = t < first || t > last ? 0xff800000u : __float_as_uint(x[j]);
             }
-            TmemStore16(score_address + 16 * piece, y);
+            TmemStore16(s_address + 16 * piece, y);
           }
           TmemStoreWait();
         }
         float most = -INFINITY;
 #pragma unroll 1
         for (int piece = 0; piece < 2; ++piece) {
-          Pair x[16];
-          TmemLoadPairs(score_address + 32 * piece, x);
-          float part[2] = {most, most};
+          float x[64];
+          TmemLoad64(s_address + 64 * piece, x);
+          float part[2] = {most, x[0]};
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float front, back;
-            SplitPair(x[j], &front, &back);
-            part[j & 1] = Max3(part[j & 1], front, back);
-          }
+          for (int j = 0; j < 64; j += 2)
+            part[j >> 1 & 1] = Max3(part[j >> 1 & 1], x[j], x[j + 1]);
           most = fmaxf(part[0], part[1]);
         }
         const bool raise = fmaf(most, factor, -top) > kRaise;
         if (__any_sync(0xffffffffu, raise)) {
           const float next = raise ? fmaf(most, factor, -kTop) : top, shrink = Exp2(top - next);
           top = next, total *= shrink;
-          if (i != 2 * begin_tile) {
-            // O as the sub-tile before left it (the one before that is done: this sub-tile's S was asked for after it)
-            alive = WarpWait(&sm.o_full[half], (outputs - 1) & 1, abort);
-            if (!alive)
-              break;
-            AfterSync();
+          if (i != begin_tile) { // the S that has just come says that the MMAs before it are done with O
 #pragma unroll 1
             for (int piece = 0; piece < D / 16; ++piece) {
-              Pair y[8];
-              TmemLoadPairs(o_address + 16 * piece, y);
+              float y[16];
+              TmemLoad16(o_address + 16 * piece, y);
               unsigned z[16];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const Pair scaled = Mul2(y[j], MakePair(shrink, shrink));
-                z[2 * j] = static_cast<unsigned>(scaled), z[2 * j + 1] = static_cast<unsigned>(scaled >> 32);
-              }
+              for (int j = 0; j < 16; ++j)
+                z[j] = __float_as_uint(y[j] * shrink);
               TmemStore16(o_address + 16 * piece, z);
             }
           }
         }
-        const Pair factors = MakePair(factor, factor), minus_top = MakePair(-top, -top);
-        Pair sum[2] = {MakePair(total, 0), MakePair(0, 0)};
+        const float2 factors = make_float2(factor, factor), minus_top = make_float2(-top, -top);
+        float2 sum[2] = {make_float2(total, 0), make_float2(0, 0)};
 #pragma unroll 1
         for (int piece = 0; piece < 2; ++piece) {
-          Pair x[16];
-          TmemLoadPairs(score_address + 32 * piece, x);
-          unsigned packed[16];
+          float x[64];
+          TmemLoad64(s_address + 64 * piece, x);
+          unsigned packed[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float p0, p1;
-            SplitPair(Fma2(x[j], factors, minus_top), &p0, &p1);
-            p0 = Exp2(p0), p1 = Exp2(p1);
-            sum[j & 1] = Add2(sum[j & 1], MakePair(p0, p1));
-            packed[j] = Pack(p0, p1);
+          for (int j = 0; j < 32; ++j) {
+            const float2 e = Fma2(make_float2(x[2 * j], x[2 * j + 1]), factors, minus_top), p = make_float2(Exp2(e.x), Exp2(e.y));
+            sum[j & 1] = Add2(sum[j & 1], p);
+            packed[j] = Pack(p.x, p.y);
           }
-          TmemStore16(score_address + 16 * piece, packed); // over scores that have been read
+          TmemStore32(s_address + 32 * piece, packed); // over scores that have been read
         }
-        float sum0, sum1;
-        SplitPair(Add2(sum[0], sum[1]), &sum0, &sum1);
-        total = sum0 + sum1;
+        sum[0] = Add2(sum[0], sum[1]);
+        total = sum[0].x + sum[0].y;
         TmemStoreWait();
         BeforeSync();
         __syncwarp();
         if (lane == 0)
-          BarrierArrive(&sm.p_full[half][sub]);
-        ++outputs, jobs += sub;
+          BarrierArrive(&sm.p_full[half]);
       }
       if (!alive)
         break;
@@ -770,13 +722,13 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
             BarrierArrive(&sm.shared_ready);
           // its O may be overwritten only when the first half has read it
           alive = WarpWait(&sm.shared_done, shared++ & 1, abort);
-          ++finished;
+          ++finished[1];
         }
         continue;
       }
       float own_weight = 1.f, other_weight = 0.f;
       if (other_half) {
-        alive = WarpWait(&sm.shared_ready, shared++ & 1, abort) && WarpWait(&sm.o_last[1], other_finished & 1, abort);
+        alive = WarpWait(&sm.shared_ready, shared++ & 1, abort) && WarpWait(&sm.o_full[1], finished[1]++ & 1, abort);
         if (!alive)
           break;
         const float2 other = sm.other[row];
@@ -784,8 +736,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         own_weight = Exp2(top - larger), other_weight = Exp2(other.x - larger);
         top = larger, total = own_weight * total + other_weight * other.y;
       }
-      other_finished += !paired || other_half;
-      alive = WarpWait(&sm.o_last[half], finished++ & 1, abort);
+      if (!paired && !half)
+        ++finished[1]; // an output that is not this half's business
+      alive = WarpWait(&sm.o_full[half], finished[half]++ & 1, abort);
       if (!alive)
         break;
       AfterSync();
@@ -848,7 +801,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         if (there)
           *reinterpret_cast<float2 *>(partial + kColumns * D + 2 * own) = make_float2(top, total);
         if (!walk.skip && tid == 0) { // the unit begins here and goes on in the next runs
-          const long long last = Quotient(walk.at + walk.unit.tiles - 1, share);
+          const long long last = Quotient(walk.at - walk.from + kSetup + walk.unit.tiles - 1, share);
           a.split[blockIdx.x] = Split{static_cast<int>(last - blockIdx.x) + 1, slot, walk.rows.begin, walk.block, walk.head, walk.unit.columns};
         }
       }
@@ -866,7 +819,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       __nanosleep(1000);
   if (warp == kMmaWarp) {
     AfterSync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
