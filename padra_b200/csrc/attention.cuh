@@ -224,7 +224,7 @@ template <typename T, int D, int Columns> int LaunchJoin(const AttentionArgs &a,
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.gridDim = dim3(grid, Columns == 256 ? 16 : 2), config.blockDim = dim3(kJoinWarps * 32), config.stream = stream;
+  config.gridDim = dim3(grid, Columns == 256 ? 16 : 4), config.blockDim = dim3(kJoinWarps * 32), config.stream = stream;
   config.attrs = &attribute, config.numAttrs = 1;
   return CudaStatus(cudaLaunchKernelEx(&config, JoinKernel<T, D, Columns>, a));
 }

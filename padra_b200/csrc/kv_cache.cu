@@ -1,11 +1,11 @@
 // Per-head norm and rotation of queries and keys, appending keys and values to the paged 4-bit cache, reading it back.
 //
 // Norm + rotation: y = x * w / sqrt(mean(x^2) + eps), then pair (a, b) -> amplitude * (a cos t - b sin t, a sin t + b cos t)
-// with t = position * inv_freq.  One pass: a head of a row sits in the registers of head_dim / 8 lanes (16 bytes of 16-bit
-// values each), the sum of squares is one value per lane and a few shuffles, and the partner of a rotated value is in the same lane
-// (interleaved) or dims / 16 lanes on (half layout).  cos and sin of a row are computed once per CTA for all of its heads:
-// the angle is reduced to a fraction of a turn in 64 bits, so a far position costs no precision and no slow path.
-// Bound by bandwidth for many rows and by launch latency for few.
+// with t = position * inv_freq.  One pass: a head of a row sits in the registers of head_dim / 8 lanes.  A warp stays with one row, so
+// that weights and the row's cos and sin stay in registers, and it has the loads of its next heads under way meanwhile, the first of them
+// from before the table is made.  cos and sin of a row are computed once per CTA for all of its heads: the angle is reduced to a
+// fraction of a turn in 64 bits, so a far position costs no precision and no slow path.
+// Bound by bandwidth for many rows and by latency for few.
 #include "kernels.cuh"
 #include "kv_cache.cuh"
 
@@ -13,67 +13,60 @@ namespace padra {
 namespace {
 
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
-constexpr int kMaxCtaRows = 4;
+constexpr int kMaxCtaRows = 4; // a row's warps: at least kRowWarps / kMaxCtaRows
 
+// Four neighbouring values of a row as they lie in memory.
 template <typename T> struct Rows;
 template <> struct Rows<__nv_bfloat16> {
-  static __device__ __forceinline__ void Load(const __nv_bfloat16 *p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  using Raw = uint2;
+  static __device__ __forceinline__ void Unpack(const Raw &u, float *x) {
+    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
+    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
   }
-  // false where a rounded value is not finite
-  template <typename Real> static __device__ __forceinline__ bool Store(__nv_bfloat16 *p, const Real (&x)[8]) {
-    unsigned w[4], wrong = 0;
+  // both blocks, rounded; false where a rounded value is not finite
+  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
+    __nv_bfloat162 p[4];
+    unsigned w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __nv_bfloat162 pair = __floats2bfloat162_rn(static_cast<float>(x[2 * i]), static_cast<float>(x[2 * i + 1]));
-      w[i] = *reinterpret_cast<const unsigned *>(&pair);
-      wrong |= ((w[i] & 0x7f80u) == 0x7f80u) | ((w[i] & 0x7f800000u) == 0x7f800000u);
+      p[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const unsigned *>(&p[i]);
     }
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    return !wrong;
+    const __nv_bfloat162 most = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+    const unsigned m = *reinterpret_cast<const unsigned *>(&most);
+    *lo = make_uint2(w[0], w[1]), *hi = make_uint2(w[2], w[3]);
+    return (m & 0x7fffu) < 0x7f80u && (m & 0x7fffffffu) < 0x7f800000u;
   }
 };
 template <> struct Rows<__half> {
-  static __device__ __forceinline__ void Load(const __half *p, float (&x)[8]) {
-    const uint4 u = *reinterpret_cast<const uint4 *>(p);
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
+  using Raw = uint2;
+  static __device__ __forceinline__ void Unpack(const Raw &u, float *x) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
   }
-  template <typename Real> static __device__ __forceinline__ bool Store(__half *p, const Real (&x)[8]) {
-    unsigned w[4], wrong = 0;
+  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
+    __half2 p[4];
+    unsigned w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const __half2 pair = __floats2half2_rn(static_cast<float>(x[2 * i]), static_cast<float>(x[2 * i + 1]));
-      w[i] = *reinterpret_cast<const unsigned *>(&pair);
-      wrong |= ((w[i] & 0x7c00u) == 0x7c00u) | ((w[i] & 0x7c000000u) == 0x7c000000u);
+      p[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const unsigned *>(&p[i]);
     }
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    return !wrong;
+    const __half2 most = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+    const unsigned m = *reinterpret_cast<const unsigned *>(&most);
+    *lo = make_uint2(w[0], w[1]), *hi = make_uint2(w[2], w[3]);
+    return (m & 0x7fffu) < 0x7c00u && (m & 0x7fffffffu) < 0x7c000000u;
   }
 };
 template <> struct Rows<float> {
-  static __device__ __forceinline__ void Load(const float *p, float (&x)[8]) {
-    const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  }
-  template <typename Real> static __device__ __forceinline__ bool Store(float *p, const Real (&x)[8]) {
+  using Raw = float4;
+  static __device__ __forceinline__ void Unpack(const Raw &u, float *x) { x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w; }
+  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
     bool fine = true;
-    float f[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = static_cast<float>(x[i]);
-      fine &= isfinite(f[i]) != 0;
-    }
-    *reinterpret_cast<float4 *>(p) = make_float4(f[0], f[1], f[2], f[3]);
-    *reinterpret_cast<float4 *>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    for (int i = 0; i < 8; ++i)
+      fine &= isfinite(x[i]) != 0;
+    *lo = make_float4(x[0], x[1], x[2], x[3]), *hi = make_float4(x[4], x[5], x[6], x[7]);
     return fine;
   }
 };
@@ -95,57 +88,6 @@ __device__ __forceinline__ void MakeTurn(double turns, double amplitude, Turn<do
   sincospi(2.0 * turns, &s, &c);
   to->cos = c * amplitude, to->sin = s * amplitude;
 }
-__device__ __forceinline__ float InverseRoot(float x) { return rsqrtf(x); }
-__device__ __forceinline__ double InverseRoot(double x) { return 1.0 / sqrt(x); }
-
-// Norm and rotation of one head held by D / 8 neighbouring lanes, eight values each.  `at` = the lane's place in the head.
-// Every lane of the warp takes part in the exchanges.
-template <int D, typename Real, typename TableReal>
-__device__ __forceinline__ void NormRotate(Real (&x)[8], int at, const unsigned short *weight, double eps, const Turn<TableReal> *turns, int dims,
-                                           bool interleaved) {
-  constexpr int kLanes = D / 8;
-  if (weight) {
-    Real sum = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      sum += x[i] * x[i];
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2)
-      sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const Real inverse = InverseRoot(sum * static_cast<Real>(1.0 / D) + static_cast<Real>(eps));
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(weight) + at);
-    const unsigned w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = x[2 * i] * inverse * static_cast<Real>(__uint_as_float(w[i] << 16));
-      x[2 * i + 1] = x[2 * i + 1] * inverse * static_cast<Real>(__uint_as_float(w[i] & 0xffff0000u));
-    }
-  }
-  if (interleaved) {
-    if (8 * at < dims) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const Turn<TableReal> t = turns[4 * at + i];
-        const Real a = x[2 * i], b = x[2 * i + 1], c = static_cast<Real>(t.cos), s = static_cast<Real>(t.sin);
-        x[2 * i] = a * c - b * s;
-        x[2 * i + 1] = a * s + b * c;
-      }
-    }
-  } else if (dims) {
-    const int half = dims / 16; // lanes between the two values of a pair
-    const bool second = at >= half;
-    const int lane = threadIdx.x & 31, from = at >= 2 * half ? lane : second ? lane - half : lane + half;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const Real other = __shfl_sync(0xffffffffu, x[i], from);
-      if (at < 2 * half) {
-        const Turn<TableReal> t = turns[8 * (second ? at - half : at) + i];
-        const Real c = static_cast<Real>(t.cos), s = static_cast<Real>(t.sin);
-        x[i] = second ? other * s + x[i] * c : x[i] * c - other * s;
-      }
-    }
-  }
-}
 
 struct HeadRows { // one of q, k, v: rows of `heads` heads
   const void *in;
@@ -160,61 +102,229 @@ struct RotaryArgs {
   int dims, interleaved;
 };
 
-// ---- norm + rotation without a cache ----
-// A CTA takes `cta_rows` rows and the heads [y * share, ...) of them; a warp takes 32 / (D / 8) heads of a row at a time.
+// ---- norm + rotation in 32 bits ----
+// A lane holds values lo .. lo+3 and hi .. hi+3 of its head, chosen so that both values of a pair are its own: no exchange but the sum's.
+struct Lane {
+  int at, lo, hi, pair; // pair: the first of its four pairs, -1 where its values are not rotated
+  bool interleaved;
+};
+template <int D> __device__ __forceinline__ Lane LaneOf(const RotaryArgs &rotary) {
+  Lane l;
+  l.at = (threadIdx.x & 31) % (D / 8), l.interleaved = rotary.interleaved;
+  const bool rotated = 8 * l.at < rotary.dims, apart = rotated && !rotary.interleaved;
+  l.lo = apart ? 4 * l.at : 8 * l.at, l.hi = apart ? rotary.dims / 2 + 4 * l.at : 8 * l.at + 4;
+  l.pair = rotated ? 4 * l.at : -1;
+  return l;
+}
+template <typename T> struct Eight { // a lane's values as they lie in memory
+  typename Rows<T>::Raw lo, hi;
+  __device__ __forceinline__ void Load(const T *head, const Lane &lane) {
+    lo = *reinterpret_cast<const typename Rows<T>::Raw *>(head + lane.lo), hi = *reinterpret_cast<const typename Rows<T>::Raw *>(head + lane.hi);
+  }
+};
+struct Weights {
+  float w[8];
+  __device__ __forceinline__ void Load(const unsigned short *weight, const Lane &lane) {
+    Rows<__nv_bfloat16>::Unpack(__ldg(reinterpret_cast<const uint2 *>(weight + lane.lo)), w);
+    Rows<__nv_bfloat16>::Unpack(__ldg(reinterpret_cast<const uint2 *>(weight + lane.hi)), w + 4);
+  }
+};
+template <int D>
+__device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool normed, const Weights &weights, float eps, const Turn<float> (&turns)[4]) {
+  if (normed) {
+    float sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      sum += x[i] * x[i];
+#pragma unroll
+    for (int d = 1; d < D / 8; d *= 2)
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const float inverse = rsqrtf(sum * (1.f / D) + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x[i] = x[i] * inverse * weights.w[i];
+  }
+  if (lane.pair < 0)
+    return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (lane.interleaved) {
+      const float a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = a * turns[i].cos - b * turns[i].sin, x[2 * i + 1] = a * turns[i].sin + b * turns[i].cos;
+    } else {
+      const float a = x[i], b = x[4 + i];
+      x[i] = a * turns[i].cos - b * turns[i].sin, x[4 + i] = a * turns[i].sin + b * turns[i].cos;
+    }
+  }
+}
+
+// Units (32 / (D / 8) heads each) first, first + step, ... of one row of q or k, by one warp; kAhead loads are under way.
+constexpr int kAhead = 4;
+template <typename T, int D> struct UnitLoop {
+  static constexpr int kSide = 32 / (D / 8);
+  Eight<T> raw[kAhead];
+  const T *in;
+  int heads, head, stride; // head: this lane's in the unit being worked on
+  __device__ __forceinline__ UnitLoop(const HeadRows &a, long long row, int first, int step, const Lane &lane)
+      : in(static_cast<const T *>(a.in) + row * a.stride), heads(a.heads), head(first * kSide + (threadIdx.x & 31) / (D / 8)), stride(step * kSide) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      Fetch(j, head + j * stride, lane);
+  }
+  __device__ __forceinline__ void Fetch(int j, int at, const Lane &lane) {
+    if (at < heads)
+      raw[j].Load(in + at * D, lane);
+  }
+  template <typename Turns>
+  __device__ __forceinline__ void Run(const HeadRows &a, long long row, const Lane &lane, float eps, const Turns &turns_of_row, int *bad) {
+    Weights weights{};
+    Turn<float> turns[4] = {};
+    if (a.weight)
+      weights.Load(a.weight, lane);
+    if (lane.pair >= 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        turns[i] = turns_of_row[lane.pair + i];
+    }
+    T *const out = static_cast<T *>(a.out) + row * a.out_stride;
+    bool fine = true;
+    const int side = (threadIdx.x & 31) / (D / 8); // the warp goes on while its first head exists
+    for (; head - side < heads;) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        if (head - side >= heads)
+          break;
+        float x[8] = {};
+        if (head < heads)
+          Rows<T>::Unpack(raw[j].lo, x), Rows<T>::Unpack(raw[j].hi, x + 4);
+        Fetch(j, head + kAhead * stride, lane);
+        NormRotate<D>(x, lane, a.weight != nullptr, weights, eps, turns);
+        if (head < heads) {
+          Eight<T> y;
+          fine &= Rows<T>::Pack(x, &y.lo, &y.hi);
+          *reinterpret_cast<typename Rows<T>::Raw *>(out + head * D + lane.lo) = y.lo;
+          *reinterpret_cast<typename Rows<T>::Raw *>(out + head * D + lane.hi) = y.hi;
+        }
+        head += stride;
+      }
+    }
+    if (!fine)
+      Raise(bad);
+  }
+};
+
+// The units of a row are dealt to its `row_warps` warps in each of gridDim.y CTAs.
+struct Share {
+  int row, first, step; // row within the CTA
+  __device__ __forceinline__ explicit Share(int row_warps) {
+    const int warp = threadIdx.x >> 5;
+    row = warp / row_warps, first = blockIdx.y * row_warps + warp % row_warps, step = row_warps * gridDim.y;
+  }
+};
+__device__ __forceinline__ int After(int first, int units, int step) { // the first of first, first + step, ... behind `units`, counted from there
+  return first >= units ? first - units : (first - units) % step + (((first - units) % step) ? step : 0);
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) NormRopeKernel(HeadRows q, HeadRows k, double eps, const int *positions, RotaryArgs rotary, int rows,
-                                                              int cta_rows, int share, int *bad) {
-  constexpr int kLanes = D / 8, kSide = 32 / kLanes;
-  __shared__ Turn<float> turns[kMaxCtaRows][D / 2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = rotary.dims / 2;
+__global__ void __launch_bounds__(kRowThreads) NormRopeKernel(HeadRows q, HeadRows k, float eps, const int *positions, RotaryArgs rotary, int rows,
+                                                              int row_warps, int *bad) {
+  constexpr int kSide = 32 / (D / 8);
+  __shared__ __align__(16) Turn<float> turns[kMaxCtaRows][D / 2];
+  const int pairs = rotary.dims / 2, cta_rows = kRowWarps / row_warps;
   const int first = blockIdx.x * cta_rows, count = min(cta_rows, rows - first);
+  const Lane lane = LaneOf<D>(rotary);
+  const Share share(row_warps);
+  const long long row = min(first + share.row, rows - 1); // a warp without a row reads the last one and stops
+  UnitLoop<T, D> q_loop(q, row, share.first, share.step, lane);
   for (int i = threadIdx.x; i < count * pairs; i += kRowThreads) {
     const int r = i / pairs, p = i - r * pairs;
     MakeTurn(Turns(positions[first + r], rotary.inv_freq[p]), rotary.amplitude, &turns[r][p]);
   }
   __syncthreads();
-  const int q_units = (q.heads + kSide - 1) / kSide, units = q_units + (k.heads + kSide - 1) / kSide;
-  const int from = blockIdx.y * share, to = min(units, from + share), mine = to - from;
-  const int at = lane % kLanes;
-  for (int i = warp; i < count * mine; i += kRowWarps) {
-    const int r = i / mine, unit = from + i - r * mine;
-    const bool is_q = unit < q_units;
-    const HeadRows &a = is_q ? q : k;
-    const int head = (is_q ? unit : unit - q_units) * kSide + lane / kLanes;
-    const bool there = head < a.heads;
-    float x[8] = {};
-    if (there)
-      Rows<T>::Load(static_cast<const T *>(a.in) + static_cast<long long>(first + r) * a.stride + head * D + 8 * at, x);
-    NormRotate<D, float>(x, at, a.weight, eps, turns[r], rotary.dims, rotary.interleaved);
-    if (there && !Rows<T>::Store(static_cast<T *>(a.out) + static_cast<long long>(first + r) * a.out_stride + head * D + 8 * at, x))
-      Raise(bad);
-  }
+  if (share.row >= count)
+    return;
+  q_loop.Run(q, row, lane, eps, turns[share.row], bad);
+  UnitLoop<T, D>(k, row, After(share.first, (q.heads + kSide - 1) / kSide, share.step), share.step, lane).Run(k, row, lane, eps, turns[share.row], bad);
 }
 
 // ---- append ----
-// Eight values of a lane as eight codes, four lanes to a group.  Everything here is 64-bit: the border between two codes is
-// met by values that a 32-bit rotation could put on either side, and equal inputs have to give equal bytes.  The FP64
-// pipe has the room: 2048 rows of four heads are a million values, some 15 operations each.
-__device__ __forceinline__ unsigned QuantiseWord(const double (&x)[8], unsigned short *scale_bits, bool *fine) {
-  double most = 0;
+// Norm and rotation of a key in 64 bits: the border between two codes is met by values that a 32-bit rotation could put on either side,
+// and equal inputs have to give equal bytes.  `at` = the lane's place in the head; it holds eight neighbouring values, the partner of
+// a rotated value is in the same lane (interleaved) or dims / 16 lanes on (half layout).  Every lane of the warp takes part.
+template <int D>
+__device__ __forceinline__ void NormRotateKey(double (&x)[8], int at, const unsigned short *weight, double eps, const Turn<double> *turns, int dims,
+                                              bool interleaved) {
+  if (weight) {
+    double sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      sum += x[i] * x[i];
+#pragma unroll
+    for (int d = 1; d < D / 8; d *= 2)
+      sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const double inverse = 1.0 / sqrt(sum * (1.0 / D) + eps);
+    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(weight) + at);
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = x[2 * i] * inverse * static_cast<double>(__uint_as_float(w[i] << 16));
+      x[2 * i + 1] = x[2 * i + 1] * inverse * static_cast<double>(__uint_as_float(w[i] & 0xffff0000u));
+    }
+  }
+  if (interleaved) {
+    if (8 * at < dims) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const Turn<double> t = turns[4 * at + i];
+        const double a = x[2 * i], b = x[2 * i + 1];
+        x[2 * i] = a * t.cos - b * t.sin;
+        x[2 * i + 1] = a * t.sin + b * t.cos;
+      }
+    }
+  } else if (dims) {
+    const int half = dims / 16; // lanes between the two values of a pair
+    const bool second = at >= half;
+    const int lane = threadIdx.x & 31, from = at >= 2 * half ? lane : second ? lane - half : lane + half;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double other = __shfl_sync(0xffffffffu, x[i], from);
+      if (at < 2 * half) {
+        const Turn<double> t = turns[8 * (second ? at - half : at) + i];
+        x[i] = second ? other * t.sin + x[i] * t.cos : x[i] * t.cos - other * t.sin;
+      }
+    }
+  }
+}
+
+// Eight values of a lane as eight codes, four lanes to a group.  The code is the nearest of x / scale, ties to even, as a division in 64
+// bits would give it, without the division: a guess in 32 bits is off by one at most (its error is far below one half), and
+// what is left of x, exact or rounded far below the difference between two inputs, decides.
+template <typename Real> __device__ __forceinline__ unsigned QuantiseWord(const Real (&x)[8], unsigned short *scale_bits, bool *fine) {
+  Real most = 0;
   bool finite = true;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    most = fmax(most, fabs(x[i]));
+    most = max(most, abs(x[i]));
     finite &= isfinite(x[i]) != 0;
   }
 #pragma unroll
   for (int d = 1; d < 4; d *= 2)
-    most = fmax(most, __shfl_xor_sync(0xffffffffu, most, d));
-  *fine = finite && most <= static_cast<double>(kKvLargest);
-  const __half h = __double2half(most / 7.0);
-  const double scale = static_cast<double>(__half2float(h));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+  *fine = finite && most <= static_cast<Real>(kKvLargest);
+  const __half h = __double2half(static_cast<double>(most) / 7.0);
+  const float scale = __half2float(h), inverse = scale > 0 ? 1.f / scale : 0.f;
+  const Real step = static_cast<Real>(scale), half = static_cast<Real>(0.5f * scale);
   unsigned word = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double code = scale > 0 ? fmin(fmax(rint(x[i] / scale), -7.0), 7.0) : 0.0;
-    word |= static_cast<unsigned>(static_cast<int>(code) + 8) << (4 * i);
+    // a scale that was rounded down may leave 7.x steps, and one below FP16's normal range many more
+    const float guess = fminf(fmaxf(rintf(static_cast<float>(x[i]) * inverse), -8.f), 8.f);
+    const Real rest = fma(-static_cast<Real>(guess), step, x[i]);
+    int code = static_cast<int>(guess);
+    const bool odd = code & 1;
+    code += (rest > half || (rest == half && odd)) - (rest < -half || (rest == -half && odd));
+    code = scale > 0 ? min(max(code, -7), 7) : 0;
+    word |= static_cast<unsigned>(code + 8) << (4 * i);
   }
   *scale_bits = __half_as_ushort(h);
   return word;
@@ -222,12 +332,29 @@ __device__ __forceinline__ unsigned QuantiseWord(const double (&x)[8], unsigned 
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, SequenceView seq, HeadRows q, HeadRows k, HeadRows v, double eps,
-                                                            RotaryArgs rotary, int cta_rows, int share, int *bad) {
+                                                            RotaryArgs rotary, int row_warps, int *bad) {
   constexpr int kLanes = D / 8, kSide = 32 / kLanes, kGroups = D / kKvGroup;
-  __shared__ Turn<double> turns[kMaxCtaRows][D / 2];
+  __shared__ __align__(16) Turn<double> turns[kMaxCtaRows][D / 2];
+  __shared__ __align__(16) Turn<float> q_turns[kMaxCtaRows][D / 2];
   __shared__ int s_page[kMaxCtaRows], s_position[kMaxCtaRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = rotary.dims / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, pairs = rotary.dims / 2, cta_rows = kRowWarps / row_warps;
   const int first = blockIdx.x * cta_rows, count = min(cta_rows, seq.rows - first);
+  const Share share(row_warps);
+  const long long row = min(first + share.row, seq.rows - 1);
+  const Lane q_lane = LaneOf<D>(rotary);
+  UnitLoop<T, D> q_loop(q, row, share.first, share.step, q_lane);
+  const int kv_units = (k.heads + kSide - 1) / kSide, at = lane % kLanes;
+  typename Rows<T>::Raw lo{}, hi{};
+  auto fetch = [&](int unit) { // K and V as they come
+    const HeadRows &a = unit < kv_units ? k : v;
+    const int head = (unit < kv_units ? unit : unit - kv_units) * kSide + lane / kLanes;
+    if (unit < 2 * kv_units && head < k.heads) {
+      const T *const from = static_cast<const T *>(a.in) + row * a.stride + head * D + 8 * at;
+      lo = *reinterpret_cast<const typename Rows<T>::Raw *>(from), hi = *reinterpret_cast<const typename Rows<T>::Raw *>(from + 4);
+    }
+  };
+  int unit = After(share.first, (q.heads + kSide - 1) / kSide, share.step);
+  fetch(unit);
   if (warp < count) {
     int position = -1, page = -1;
     const int s = LocateRow(seq, cache, first + warp, &position, bad);
@@ -239,39 +366,38 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
   __syncthreads();
   for (int i = threadIdx.x; i < count * pairs; i += kRowThreads) {
     const int r = i / pairs, p = i - r * pairs;
-    if (s_page[r] >= 0)
-      MakeTurn(Turns(s_position[r], rotary.inv_freq[p]), rotary.amplitude, &turns[r][p]);
+    if (s_page[r] >= 0) {
+      Turn<double> turn;
+      MakeTurn(Turns(s_position[r], rotary.inv_freq[p]), rotary.amplitude, &turn);
+      turns[r][p] = turn, q_turns[r][p] = Turn<float>{static_cast<float>(turn.cos), static_cast<float>(turn.sin)};
+    }
   }
   __syncthreads();
-  const int q_units = (q.heads + kSide - 1) / kSide, kv_units = (k.heads + kSide - 1) / kSide, units = q_units + 2 * kv_units;
-  const int from = blockIdx.y * share, to = min(units, from + share), mine = to - from;
-  const int at = lane % kLanes;
-  for (int i = warp; i < count * mine; i += kRowWarps) { // warp-uniform up to the head
-    const int r = i / mine, unit = from + i - r * mine;
-    if (s_page[r] < 0)
-      continue;
-    const int kind = unit < q_units ? 0 : unit < q_units + kv_units ? 1 : 2;
-    const HeadRows &a = kind == 0 ? q : kind == 1 ? k : v;
-    const int head = (kind == 0 ? unit : unit - q_units - (kind - 1) * kv_units) * kSide + lane / kLanes;
-    const bool there = head < a.heads;
+  if (share.row >= count || s_page[share.row] < 0)
+    return;
+  q_loop.Run(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
+  const int slot = s_position[share.row] & (cache.page_size - 1), group = at / 4, quarter = at & 3;
+  for (; unit < 2 * kv_units; unit += share.step) { // warp-uniform up to the head
+    const bool is_v = unit >= kv_units;
+    const int head = (is_v ? unit - kv_units : unit) * kSide + lane / kLanes;
+    const bool there = head < k.heads;
     float x[8] = {};
     if (there)
-      Rows<T>::Load(static_cast<const T *>(a.in) + static_cast<long long>(first + r) * a.stride + head * D + 8 * at, x);
-    if (kind == 0) {
-      NormRotate<D, float>(x, at, a.weight, eps, turns[r], rotary.dims, rotary.interleaved);
-      if (there && !Rows<T>::Store(static_cast<T *>(a.out) + static_cast<long long>(first + r) * a.out_stride + head * D + 8 * at, x))
-        Raise(bad);
-      continue;
-    }
-    double y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      y[j] = static_cast<double>(x[j]);
-    if (kind == 1)
-      NormRotate<D, double>(y, at, a.weight, eps, turns[r], rotary.dims, rotary.interleaved);
+      Rows<T>::Unpack(lo, x), Rows<T>::Unpack(hi, x + 4);
+    fetch(unit + share.step);
     unsigned short scale;
     bool fine;
-    const unsigned word = QuantiseWord(y, &scale, &fine);
+    unsigned word;
+    if (is_v) { // 24 bits at most: a multiple of half a scale is exact in 32
+      word = QuantiseWord(x, &scale, &fine);
+    } else {
+      double y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        y[j] = static_cast<double>(x[j]);
+      NormRotateKey<D>(y, at, k.weight, eps, turns[share.row], rotary.dims, rotary.interleaved);
+      word = QuantiseWord(y, &scale, &fine);
+    }
     // one decision for the whole head: it is written or left as it was
     const unsigned lanes = (kLanes == 32 ? 0xffffffffu : (1u << kLanes) - 1) << (lane / kLanes * kLanes);
     const bool whole = (__ballot_sync(0xffffffffu, !fine) & lanes) == 0;
@@ -281,8 +407,7 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
       Raise(bad);
       continue;
     }
-    const int slot = s_position[r] & (cache.page_size - 1), group = at / 4, quarter = at & 3;
-    unsigned char *codes = cache.block(s_page[r], head) + (kind == 2 ? cache.code_bytes() + cache.scale_bytes() : 0);
+    unsigned char *codes = cache.block(s_page[share.row], head) + (is_v ? cache.code_bytes() + cache.scale_bytes() : 0);
     reinterpret_cast<unsigned *>(codes + slot * (D / 2))[quarter * kGroups + group] = word;
     if (!quarter)
       reinterpret_cast<unsigned short *>(codes + cache.code_bytes() + slot * (D / 16))[group] = scale;
@@ -291,7 +416,7 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
 
 // ---- read ----
 // A thread takes one word (eight codes) of K and of V of one head.
-constexpr int kReadRows = 16;
+constexpr int kReadRows = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, SequenceView seq, T *k_out, T *v_out, long long k_stride, long long v_stride,
                                                           int *bad) {
@@ -299,13 +424,13 @@ __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, Sequence
   __shared__ int s_page[kReadRows], s_slot[kReadRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = blockIdx.x * kReadRows, count = min(kReadRows, seq.rows - first);
-  for (int r = warp; r < count; r += kRowWarps) {
+  if (warp < count) {
     int position = -1, page = -1;
-    const int s = LocateRow(seq, cache, first + r, &position, bad);
+    const int s = LocateRow(seq, cache, first + warp, &position, bad);
     if (s >= 0 && position >= 0)
       page = PageOf(seq, cache, s, position, bad);
     if (!lane)
-      s_page[r] = page, s_slot[r] = position & (cache.page_size - 1);
+      s_page[warp] = page, s_slot[warp] = position & (cache.page_size - 1);
   }
   __syncthreads();
   const int per_row = cache.kv_heads * kWords;
@@ -313,34 +438,43 @@ __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, Sequence
     const int r = i / per_row, j = i - r * per_row, head = j / kWords, at = j % kWords; // values 8 at .. 8 at + 7 of the head
     if (s_page[r] < 0)
       continue;
-    const unsigned char *codes = cache.block(s_page[r], head);
-    const int group = at / 4, place = (at & 3) * kGroups + group;
+    const unsigned char *const codes = cache.block(s_page[r], head);
+    const int group = at / 4, place = (at & 3) * kGroups + group, second = cache.code_bytes() + cache.scale_bytes();
+    unsigned word[2];
+    unsigned short scale[2];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) { // all loads first
+      word[which] = reinterpret_cast<const unsigned *>(codes + which * second + s_slot[r] * (D / 2))[place];
+      scale[which] = reinterpret_cast<const unsigned short *>(codes + which * second + cache.code_bytes() + s_slot[r] * (D / 16))[group];
+    }
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      const unsigned word = reinterpret_cast<const unsigned *>(codes + s_slot[r] * (D / 2))[place];
-      const float scale = HalfBitsToFloat(reinterpret_cast<const unsigned short *>(codes + cache.code_bytes() + s_slot[r] * (D / 16))[group]);
+      const float step = HalfBitsToFloat(scale[which]);
       float x[8];
 #pragma unroll
       for (int n = 0; n < 8; ++n)
-        x[n] = static_cast<float>(static_cast<int>(word >> (4 * n) & 15u) - 8) * scale;
-      T *out = which ? v_out + (first + r) * v_stride : k_out + (first + r) * k_stride;
-      if (!Rows<T>::Store(out + head * D + 8 * at, x))
+        x[n] = static_cast<float>(static_cast<int>(word[which] >> (4 * n) & 15u) - 8) * step;
+      T *const out = (which ? v_out + (first + r) * v_stride : k_out + (first + r) * k_stride) + head * D + 8 * at;
+      Eight<T> y;
+      if (!Rows<T>::Pack(x, &y.lo, &y.hi))
         Raise(bad);
-      codes += cache.code_bytes() + cache.scale_bytes();
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4 *>(out) = make_uint4(y.lo.x, y.lo.y, y.hi.x, y.hi.y);
+      } else {
+        *reinterpret_cast<float4 *>(out) = y.lo, *reinterpret_cast<float4 *>(out + 4) = y.hi;
+      }
     }
   }
 }
 
-// Rows per CTA and heads per CTA: four rows share a CTA's cos and sin where there are rows for every SM anyway; few rows are
-// spread over the SMs by splitting their heads, one warp's share each at the least.
-void Shape(int rows, int units, int *cta_rows, dim3 *grid, int *share) {
-  *cta_rows = rows >= 4 * 148 ? 4 : 1;
-  const int x = (rows + *cta_rows - 1) / *cta_rows;
-  int parts = *cta_rows > 1 ? 1 : (2 * 148 + x - 1) / x;
-  const int most = (units + kRowWarps - 1) / kRowWarps;
-  parts = parts < 1 ? 1 : parts > most ? most : parts;
-  *share = (units + parts - 1) / parts;
-  *grid = dim3(x, (units + *share - 1) / *share);
+// Warps per row and CTAs per row: four rows share a CTA where there are rows for every SM anyway; few rows are spread over the SMs by
+// splitting their heads, one unit per warp at the least.
+void Shape(int rows, int units, int *row_warps, dim3 *grid) {
+  const int cta_rows = rows >= 4 * 148 ? kMaxCtaRows : 1;
+  *row_warps = kRowWarps / cta_rows;
+  const int x = (rows + cta_rows - 1) / cta_rows, most = (units + *row_warps - 1) / *row_warps;
+  int parts = cta_rows > 1 ? 1 : (2 * 148 + x - 1) / x;
+  *grid = dim3(x, parts < 1 ? 1 : parts > most ? most : parts);
 }
 
 template <template <typename, int> class Op, typename T, typename... A> int ByDim(int head_dim, const A &...a) {
@@ -371,10 +505,10 @@ template <typename T, int D> struct NormRope {
   static int Run(const HeadRows &q, const HeadRows &k, double eps, const int *positions, const RotaryArgs &rotary, int rows, int *bad,
                  cudaStream_t stream) {
     constexpr int kSide = 32 / (D / 8);
-    int cta_rows, share;
+    int row_warps;
     dim3 grid;
-    Shape(rows, (q.heads + kSide - 1) / kSide + (k.heads + kSide - 1) / kSide, &cta_rows, &grid, &share);
-    NormRopeKernel<T, D><<<grid, kRowThreads, 0, stream>>>(q, k, eps, positions, rotary, rows, cta_rows, share, bad);
+    Shape(rows, (q.heads + kSide - 1) / kSide + (k.heads + kSide - 1) / kSide, &row_warps, &grid);
+    NormRopeKernel<T, D><<<grid, kRowThreads, 0, stream>>>(q, k, static_cast<float>(eps), positions, rotary, rows, row_warps, bad);
     return CudaStatus(cudaGetLastError());
   }
 };
@@ -383,10 +517,10 @@ template <typename T, int D> struct Append {
   static int Run(const KvView &cache, const SequenceView &seq, const HeadRows &q, const HeadRows &k, const HeadRows &v, double eps,
                  const RotaryArgs &rotary, int *bad, cudaStream_t stream) {
     constexpr int kSide = 32 / (D / 8);
-    int cta_rows, share;
+    int row_warps;
     dim3 grid;
-    Shape(seq.rows, (q.heads + kSide - 1) / kSide + 2 * ((k.heads + kSide - 1) / kSide), &cta_rows, &grid, &share);
-    AppendKernel<T, D><<<grid, kRowThreads, 0, stream>>>(cache, seq, q, k, v, eps, rotary, cta_rows, share, bad);
+    Shape(seq.rows, (q.heads + kSide - 1) / kSide + 2 * ((k.heads + kSide - 1) / kSide), &row_warps, &grid);
+    AppendKernel<T, D><<<grid, kRowThreads, 0, stream>>>(cache, seq, q, k, v, eps, rotary, row_warps, bad);
     return CudaStatus(cudaGetLastError());
   }
 };

@@ -66,6 +66,7 @@ __device__ __forceinline__ bool SequenceRows(const SequenceView &v, const KvView
 __device__ __forceinline__ int LocateRow(const SequenceView &v, const KvView &cache, int row, int *position, int *bad) {
   const int lane = threadIdx.x & 31;
   int s = 0; // sequences that end at or before `row`
+#pragma unroll 4
   for (int i = 0; i < v.count; i += 32) {
     const bool before = i + lane < v.count && v.row_begin[i + lane + 1] <= row;
     s += __popc(__ballot_sync(0xffffffffu, before));
