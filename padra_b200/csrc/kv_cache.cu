@@ -5,7 +5,7 @@
 // that weights and the row's cos and sin stay in registers, and it has the loads of its next heads under way meanwhile, the first of them
 // from before the table is made.  cos and sin of a row are computed once per CTA for all of its heads: the angle is reduced to a
 // fraction of a turn in 64 bits, so a far position costs no precision and no slow path.
-// Bound by bandwidth for many rows and by latency for few.
+// Bound by bandwidth for many rows (16384 rows of 32 + 4 heads of 128 in FP16: 62 us, 4.9 TB/s) and by latency for few (one row: 2.7 us).
 #include "kernels.cuh"
 #include "kv_cache.cuh"
 
@@ -13,7 +13,7 @@ namespace padra {
 namespace {
 
 constexpr int kRowThreads = 256, kRowWarps = kRowThreads / 32;
-constexpr int kMaxCtaRows = 4; // a row's warps: at least kRowWarps / kMaxCtaRows
+constexpr int kMaxCtaRows = kRowWarps;
 
 // Four neighbouring values of a row as they lie in memory.
 template <typename T> struct Rows;
@@ -23,8 +23,15 @@ template <> struct Rows<__nv_bfloat16> {
     x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
     x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
   }
-  // both blocks, rounded; false where a rounded value is not finite
-  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
+  // Largest magnitude of the rounded values so far, two at a time; an infinity or a NaN stays.
+  struct Most {
+    __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+    __device__ __forceinline__ bool Finite() const {
+      const unsigned u = *reinterpret_cast<const unsigned *>(&m);
+      return (u & 0x7fffu) < 0x7f80u && (u & 0x7fffffffu) < 0x7f800000u;
+    }
+  };
+  static __device__ __forceinline__ void Pack(const float (&x)[8], Raw *lo, Raw *hi, Most *most) {
     __nv_bfloat162 p[4];
     unsigned w[4];
 #pragma unroll
@@ -32,10 +39,10 @@ template <> struct Rows<__nv_bfloat16> {
       p[i] = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
       w[i] = *reinterpret_cast<const unsigned *>(&p[i]);
     }
-    const __nv_bfloat162 most = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
-    const unsigned m = *reinterpret_cast<const unsigned *>(&most);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      most->m = __hmax2_nan(most->m, __habs2(p[i]));
     *lo = make_uint2(w[0], w[1]), *hi = make_uint2(w[2], w[3]);
-    return (m & 0x7fffu) < 0x7f80u && (m & 0x7fffffffu) < 0x7f800000u;
   }
 };
 template <> struct Rows<__half> {
@@ -44,7 +51,14 @@ template <> struct Rows<__half> {
     const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
     x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
   }
-  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
+  struct Most {
+    __half2 m = __floats2half2_rn(0.f, 0.f);
+    __device__ __forceinline__ bool Finite() const {
+      const unsigned u = *reinterpret_cast<const unsigned *>(&m);
+      return (u & 0x7fffu) < 0x7c00u && (u & 0x7fffffffu) < 0x7c000000u;
+    }
+  };
+  static __device__ __forceinline__ void Pack(const float (&x)[8], Raw *lo, Raw *hi, Most *most) {
     __half2 p[4];
     unsigned w[4];
 #pragma unroll
@@ -52,22 +66,24 @@ template <> struct Rows<__half> {
       p[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
       w[i] = *reinterpret_cast<const unsigned *>(&p[i]);
     }
-    const __half2 most = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
-    const unsigned m = *reinterpret_cast<const unsigned *>(&most);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      most->m = __hmax2_nan(most->m, __habs2(p[i]));
     *lo = make_uint2(w[0], w[1]), *hi = make_uint2(w[2], w[3]);
-    return (m & 0x7fffu) < 0x7c00u && (m & 0x7fffffffu) < 0x7c000000u;
   }
 };
 template <> struct Rows<float> {
   using Raw = float4;
   static __device__ __forceinline__ void Unpack(const Raw &u, float *x) { x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w; }
-  static __device__ __forceinline__ bool Pack(const float (&x)[8], Raw *lo, Raw *hi) {
-    bool fine = true;
+  struct Most {
+    float m = 0; // zero times each value: NaN once one was not finite
+    __device__ __forceinline__ bool Finite() const { return m == 0.f; }
+  };
+  static __device__ __forceinline__ void Pack(const float (&x)[8], Raw *lo, Raw *hi, Most *most) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      fine &= isfinite(x[i]) != 0;
+      most->m = fmaf(x[i], 0.f, most->m);
     *lo = make_float4(x[0], x[1], x[2], x[3]), *hi = make_float4(x[4], x[5], x[6], x[7]);
-    return fine;
   }
 };
 
@@ -106,11 +122,10 @@ struct RotaryArgs {
 // A lane holds values lo .. lo+3 and hi .. hi+3 of its head, chosen so that both values of a pair are its own: no exchange but the sum's.
 struct Lane {
   int at, lo, hi, pair; // pair: the first of its four pairs, -1 where its values are not rotated
-  bool interleaved;
 };
 template <int D> __device__ __forceinline__ Lane LaneOf(const RotaryArgs &rotary) {
   Lane l;
-  l.at = (threadIdx.x & 31) % (D / 8), l.interleaved = rotary.interleaved;
+  l.at = (threadIdx.x & 31) % (D / 8);
   const bool rotated = 8 * l.at < rotary.dims, apart = rotated && !rotary.interleaved;
   l.lo = apart ? 4 * l.at : 8 * l.at, l.hi = apart ? rotary.dims / 2 + 4 * l.at : 8 * l.at + 4;
   l.pair = rotated ? 4 * l.at : -1;
@@ -129,7 +144,7 @@ struct Weights {
     Rows<__nv_bfloat16>::Unpack(__ldg(reinterpret_cast<const uint2 *>(weight + lane.hi)), w + 4);
   }
 };
-template <int D>
+template <int D, bool Interleaved>
 __device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool normed, const Weights &weights, float eps, const Turn<float> (&turns)[4]) {
   if (normed) {
     float sum = 0;
@@ -148,7 +163,7 @@ __device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool
     return;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (lane.interleaved) {
+    if (Interleaved) {
       const float a = x[2 * i], b = x[2 * i + 1];
       x[2 * i] = a * turns[i].cos - b * turns[i].sin, x[2 * i + 1] = a * turns[i].sin + b * turns[i].cos;
     } else {
@@ -158,57 +173,61 @@ __device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool
   }
 }
 
-// Units (32 / (D / 8) heads each) first, first + step, ... of one row of q or k, by one warp; kAhead loads are under way.
-constexpr int kAhead = 4;
-template <typename T, int D> struct UnitLoop {
+// Units (32 / (D / 8) heads each) first, first + step, ... of one row of q or k, by one warp; Ahead loads are under way.
+template <typename T, int D, int Ahead> struct UnitLoop {
   static constexpr int kSide = 32 / (D / 8);
-  Eight<T> raw[kAhead];
-  const T *in;
-  int heads, head, stride; // head: this lane's in the unit being worked on
+  Eight<T> raw[Ahead];
+  const T *in;                  // this lane's values of the next unit to be loaded
+  int head, heads, stride, left; // the unit being worked on: this lane's head; units to do
   __device__ __forceinline__ UnitLoop(const HeadRows &a, long long row, int first, int step, const Lane &lane)
-      : in(static_cast<const T *>(a.in) + row * a.stride), heads(a.heads), head(first * kSide + (threadIdx.x & 31) / (D / 8)), stride(step * kSide) {
+      : head(first * kSide + (threadIdx.x & 31) / (D / 8)), heads(a.heads), stride(step * kSide) {
+    const int units = (heads + kSide - 1) / kSide;
+    left = first < units ? (units - first + step - 1) / step : 0;
+    in = static_cast<const T *>(a.in) + row * a.stride + head * D;
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
+    for (int j = 0; j < Ahead; ++j) {
+      raw[j] = Eight<T>{};
       Fetch(j, head + j * stride, lane);
+    }
   }
   __device__ __forceinline__ void Fetch(int j, int at, const Lane &lane) {
     if (at < heads)
-      raw[j].Load(in + at * D, lane);
+      raw[j].Load(in, lane);
+    in += stride * D;
   }
-  template <typename Turns>
+  template <bool Interleaved, typename Turns>
   __device__ __forceinline__ void Run(const HeadRows &a, long long row, const Lane &lane, float eps, const Turns &turns_of_row, int *bad) {
     Weights weights{};
     Turn<float> turns[4] = {};
-    if (a.weight)
+    const bool normed = a.weight != nullptr;
+    if (normed)
       weights.Load(a.weight, lane);
     if (lane.pair >= 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         turns[i] = turns_of_row[lane.pair + i];
     }
-    T *const out = static_cast<T *>(a.out) + row * a.out_stride;
-    bool fine = true;
-    const int side = (threadIdx.x & 31) / (D / 8); // the warp goes on while its first head exists
-    for (; head - side < heads;) {
+    T *out = static_cast<T *>(a.out) + row * a.out_stride + head * D;
+    typename Rows<T>::Most most;
+    for (; left > 0; left -= Ahead) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        if (head - side >= heads)
+      for (int j = 0; j < Ahead; ++j) {
+        if (j >= left)
           break;
-        float x[8] = {};
-        if (head < heads)
-          Rows<T>::Unpack(raw[j].lo, x), Rows<T>::Unpack(raw[j].hi, x + 4);
-        Fetch(j, head + kAhead * stride, lane);
-        NormRotate<D>(x, lane, a.weight != nullptr, weights, eps, turns);
+        float x[8];
+        Rows<T>::Unpack(raw[j].lo, x), Rows<T>::Unpack(raw[j].hi, x + 4);
+        Fetch(j, head + Ahead * stride, lane);
+        NormRotate<D, Interleaved>(x, lane, normed, weights, eps, turns);
         if (head < heads) {
           Eight<T> y;
-          fine &= Rows<T>::Pack(x, &y.lo, &y.hi);
-          *reinterpret_cast<typename Rows<T>::Raw *>(out + head * D + lane.lo) = y.lo;
-          *reinterpret_cast<typename Rows<T>::Raw *>(out + head * D + lane.hi) = y.hi;
+          Rows<T>::Pack(x, &y.lo, &y.hi, &most);
+          *reinterpret_cast<typename Rows<T>::Raw *>(out + lane.lo) = y.lo;
+          *reinterpret_cast<typename Rows<T>::Raw *>(out + lane.hi) = y.hi;
         }
-        head += stride;
+        head += stride, out += stride * D;
       }
     }
-    if (!fine)
+    if (!most.Finite())
       Raise(bad);
   }
 };
@@ -235,7 +254,7 @@ __global__ void __launch_bounds__(kRowThreads) NormRopeKernel(HeadRows q, HeadRo
   const Lane lane = LaneOf<D>(rotary);
   const Share share(row_warps);
   const long long row = min(first + share.row, rows - 1); // a warp without a row reads the last one and stops
-  UnitLoop<T, D> q_loop(q, row, share.first, share.step, lane);
+  UnitLoop<T, D, 4> q_loop(q, row, share.first, share.step, lane);
   for (int i = threadIdx.x; i < count * pairs; i += kRowThreads) {
     const int r = i / pairs, p = i - r * pairs;
     MakeTurn(Turns(positions[first + r], rotary.inv_freq[p]), rotary.amplitude, &turns[r][p]);
@@ -243,8 +262,14 @@ __global__ void __launch_bounds__(kRowThreads) NormRopeKernel(HeadRows q, HeadRo
   __syncthreads();
   if (share.row >= count)
     return;
-  q_loop.Run(q, row, lane, eps, turns[share.row], bad);
-  UnitLoop<T, D>(k, row, After(share.first, (q.heads + kSide - 1) / kSide, share.step), share.step, lane).Run(k, row, lane, eps, turns[share.row], bad);
+  UnitLoop<T, D, 2> k_loop(k, row, After(share.first, (q.heads + kSide - 1) / kSide, share.step), share.step, lane);
+  if (rotary.interleaved) {
+    q_loop.template Run<true>(q, row, lane, eps, turns[share.row], bad);
+    k_loop.template Run<true>(k, row, lane, eps, turns[share.row], bad);
+  } else {
+    q_loop.template Run<false>(q, row, lane, eps, turns[share.row], bad);
+    k_loop.template Run<false>(k, row, lane, eps, turns[share.row], bad);
+  }
 }
 
 // ---- append ----
@@ -342,7 +367,7 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
   const Share share(row_warps);
   const long long row = min(first + share.row, seq.rows - 1);
   const Lane q_lane = LaneOf<D>(rotary);
-  UnitLoop<T, D> q_loop(q, row, share.first, share.step, q_lane);
+  UnitLoop<T, D, 2> q_loop(q, row, share.first, share.step, q_lane);
   const int kv_units = (k.heads + kSide - 1) / kSide, at = lane % kLanes;
   typename Rows<T>::Raw lo{}, hi{};
   auto fetch = [&](int unit) { // K and V as they come
@@ -375,7 +400,10 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
   __syncthreads();
   if (share.row >= count || s_page[share.row] < 0)
     return;
-  q_loop.Run(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
+  if (rotary.interleaved)
+    q_loop.template Run<true>(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
+  else
+    q_loop.template Run<false>(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
   const int slot = s_position[share.row] & (cache.page_size - 1), group = at / 4, quarter = at & 3;
   for (; unit < 2 * kv_units; unit += share.step) { // warp-uniform up to the head
     const bool is_v = unit >= kv_units;
@@ -415,62 +443,65 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
 }
 
 // ---- read ----
-// A thread takes one word (eight codes) of K and of V of one head.
-constexpr int kReadRows = 4;
+// A warp takes one row; a lane one word (eight codes) of K and of V of one head at a time, two of each with all loads first.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, SequenceView seq, T *k_out, T *v_out, long long k_stride, long long v_stride,
                                                           int *bad) {
-  constexpr int kWords = D / 8, kGroups = D / kKvGroup;
-  __shared__ int s_page[kReadRows], s_slot[kReadRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int first = blockIdx.x * kReadRows, count = min(kReadRows, seq.rows - first);
-  if (warp < count) {
-    int position = -1, page = -1;
-    const int s = LocateRow(seq, cache, first + warp, &position, bad);
-    if (s >= 0 && position >= 0)
-      page = PageOf(seq, cache, s, position, bad);
-    if (!lane)
-      s_page[warp] = page, s_slot[warp] = position & (cache.page_size - 1);
-  }
-  __syncthreads();
-  const int per_row = cache.kv_heads * kWords;
-  for (int i = threadIdx.x; i < count * per_row; i += kRowThreads) {
-    const int r = i / per_row, j = i - r * per_row, head = j / kWords, at = j % kWords; // values 8 at .. 8 at + 7 of the head
-    if (s_page[r] < 0)
-      continue;
-    const unsigned char *const codes = cache.block(s_page[r], head);
-    const int group = at / 4, place = (at & 3) * kGroups + group, second = cache.code_bytes() + cache.scale_bytes();
-    unsigned word[2];
-    unsigned short scale[2];
+  constexpr int kWords = D / 8, kGroups = D / kKvGroup, kFlight = 4;
+  const int lane = threadIdx.x & 31, row = blockIdx.x * kRowWarps + (threadIdx.x >> 5);
+  if (row >= seq.rows)
+    return;
+  int position = -1;
+  const int s = LocateRow(seq, cache, row, &position, bad);
+  const int page = s >= 0 && position >= 0 ? PageOf(seq, cache, s, position, bad) : -1;
+  if (page < 0)
+    return;
+  const int words = cache.kv_heads * kWords, block_bytes = cache.block_bytes(), second = cache.code_bytes() + cache.scale_bytes();
+  const int slot = position & (cache.page_size - 1), at = lane % kWords, group = at / 4, place = (at & 3) * kGroups + group;
+  const unsigned char *const codes = cache.block(page, 0) + slot * (D / 2) + 4 * place;
+  const unsigned char *const scales = cache.block(page, 0) + cache.code_bytes() + slot * (D / 16) + 2 * group;
+  typename Rows<T>::Most most;
+  for (int j0 = lane; j0 < words; j0 += 16 * kFlight) {
+    unsigned word[kFlight];
+    unsigned short scale[kFlight];
 #pragma unroll
-    for (int which = 0; which < 2; ++which) { // all loads first
-      word[which] = reinterpret_cast<const unsigned *>(codes + which * second + s_slot[r] * (D / 2))[place];
-      scale[which] = reinterpret_cast<const unsigned short *>(codes + which * second + cache.code_bytes() + s_slot[r] * (D / 16))[group];
+    for (int i = 0; i < kFlight; ++i) { // K and V in turn; word j of the row is word `at` of head j / kWords
+      const int j = j0 + i / 2 * 32;
+      if (j < words) {
+        const long long offset = static_cast<long long>(j / kWords) * block_bytes + i % 2 * second;
+        word[i] = *reinterpret_cast<const unsigned *>(codes + offset);
+        scale[i] = *reinterpret_cast<const unsigned short *>(scales + offset);
+      }
     }
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const float step = HalfBitsToFloat(scale[which]);
-      float x[8];
+    for (int i = 0; i < kFlight; ++i) {
+      const int j = j0 + i / 2 * 32;
+      if (j < words) {
+        const float step = HalfBitsToFloat(scale[i]);
+        float x[8];
 #pragma unroll
-      for (int n = 0; n < 8; ++n)
-        x[n] = static_cast<float>(static_cast<int>(word[which] >> (4 * n) & 15u) - 8) * step;
-      T *const out = (which ? v_out + (first + r) * v_stride : k_out + (first + r) * k_stride) + head * D + 8 * at;
-      Eight<T> y;
-      if (!Rows<T>::Pack(x, &y.lo, &y.hi))
-        Raise(bad);
-      if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4 *>(out) = make_uint4(y.lo.x, y.lo.y, y.hi.x, y.hi.y);
-      } else {
-        *reinterpret_cast<float4 *>(out) = y.lo, *reinterpret_cast<float4 *>(out + 4) = y.hi;
+        for (int n = 0; n < 8; ++n) // 2^23 + code as a float's bits, less 2^23 + 8
+          x[n] = (__uint_as_float(0x4b000000u | (word[i] >> (4 * n) & 15u)) - 8388616.f) * step;
+        T *const out = (i % 2 ? v_out + row * v_stride : k_out + row * k_stride) + 8 * j;
+        Eight<T> y;
+        Rows<T>::Pack(x, &y.lo, &y.hi, &most);
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4 *>(out) = make_uint4(y.lo.x, y.lo.y, y.hi.x, y.hi.y);
+        } else {
+          *reinterpret_cast<float4 *>(out) = y.lo, *reinterpret_cast<float4 *>(out + 4) = y.hi;
+        }
       }
     }
   }
+  if (!most.Finite())
+    Raise(bad);
 }
 
-// Warps per row and CTAs per row: four rows share a CTA where there are rows for every SM anyway; few rows are spread over the SMs by
-// splitting their heads, one unit per warp at the least.
+// Warps per row and CTAs per row: a warp takes a row whole where that fills the SMs twice over (16384 rows of 36 heads: 62 us, against
+// 69 us with two warps to a row, since fewer warps wait for tables); few rows are spread over the SMs by splitting their
+// heads, one unit per warp at the least.
 void Shape(int rows, int units, int *row_warps, dim3 *grid) {
-  const int cta_rows = rows >= 4 * 148 ? kMaxCtaRows : 1;
+  const int cta_rows = rows >= 2 * 148 * kMaxCtaRows ? kMaxCtaRows : rows >= 4 * 148 ? 4 : 1;
   *row_warps = kRowWarps / cta_rows;
   const int x = (rows + cta_rows - 1) / cta_rows, most = (units + *row_warps - 1) / *row_warps;
   int parts = cta_rows > 1 ? 1 : (2 * 148 + x - 1) / x;
@@ -528,7 +559,7 @@ template <typename T, int D> struct Read {
   static constexpr int kWidest = 128;
   static int Run(const KvView &cache, const SequenceView &seq, void *k_out, void *v_out, long long k_stride, long long v_stride, int *bad,
                  cudaStream_t stream) {
-    ReadKernel<T, D><<<(seq.rows + kReadRows - 1) / kReadRows, kRowThreads, 0, stream>>>(cache, seq, static_cast<T *>(k_out), static_cast<T *>(v_out),
+    ReadKernel<T, D><<<(seq.rows + kRowWarps - 1) / kRowWarps, kRowThreads, 0, stream>>>(cache, seq, static_cast<T *>(k_out), static_cast<T *>(v_out),
                                                                                        k_stride, v_stride, bad);
     return CudaStatus(cudaGetLastError());
   }
