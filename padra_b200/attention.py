@@ -46,6 +46,7 @@ class KvCache:
               "pool is a contiguous uint8 tensor [pages][kv_heads][block bytes]")
         self.pool, self.page_size, self.head_dim = pool, page_size, head_dim
         self.pages, self.kv_heads = pool.shape[:2]
+        self.device_index = pool.get_device()
         self.struct = B.KvCacheStruct(pool.data_ptr(), self.pages, page_size, self.kv_heads, head_dim)
         self.ref = C.addressof(self.struct)
 
@@ -61,6 +62,7 @@ class Sequences:
             _need(t.dtype == torch.int32 and t.is_contiguous() and t.device == context.device, "page_table, row_begin and context are contiguous int32 tensors of one device")
         _need(page_table.dim() == 2 and page_table.shape[0] == count and row_begin.numel() == count + 1, "page_table [count][stride], row_begin [count + 1], context [count]")
         self.page_table, self.row_begin, self.context, self.rows, self.max_rows = page_table, row_begin, context, rows, max_rows
+        self.device_index = context.get_device()
         self.struct = B.SequencesStruct(page_table.data_ptr(), row_begin.data_ptr(), context.data_ptr(), count, page_table.shape[1], rows, max_rows)
         self.ref = C.addressof(self.struct)
 
@@ -71,13 +73,16 @@ class Rotary:
     def __init__(self, inv_freq: torch.Tensor, interleaved: bool = False, amplitude: float = 1.0):
         _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous(), "inv_freq is a contiguous float64 vector")
         self.inv_freq = inv_freq
+        self.device_index = inv_freq.get_device()
         self.struct = B.RotaryStruct(inv_freq.data_ptr(), amplitude, 2 * inv_freq.numel(), int(interleaved))
         self.ref = C.addressof(self.struct)
 
 
-def _row_stride(x: torch.Tensor, rows: int, dim: int, dtype: torch.dtype, what: str) -> int:
-    """Checks a [rows][heads][dim] row array, whose heads lie side by side, and returns its stride per row."""
+def _row_stride(x: torch.Tensor, rows: int, dim: int, dtype: torch.dtype, what: str, device: int) -> int:
+    """Checks a [rows][heads][dim] row array on a device, whose heads lie side by side, and returns its stride per row."""
     shape = x.shape
+    if x.get_device() != device:
+        raise ValueError(f"{what}: on {x.device}, wanted cuda:{device}")
     if len(shape) != 3 or shape[0] != rows or shape[2] != dim or x.dtype is not dtype:
         raise ValueError(f"{what}: want [{rows}][heads][{dim}] of {dtype}, got {list(shape)} of {x.dtype}")
     if x.is_contiguous():
@@ -88,11 +93,11 @@ def _row_stride(x: torch.Tensor, rows: int, dim: int, dtype: torch.dtype, what: 
     return stride[0]
 
 
-def _weight(w: torch.Tensor | None, dim: int) -> int | None:
+def _weight(w: torch.Tensor | None, dim: int, device: int) -> int | None:
     if w is None:
         return None
-    if (w.dtype is not torch.bfloat16 and w.dtype is not torch.uint16) or w.numel() != dim or not w.is_contiguous():
-        raise ValueError("norm weights are BF16 vectors of head_dim values")
+    if w.get_device() != device or (w.dtype is not torch.bfloat16 and w.dtype is not torch.uint16) or w.numel() != dim or not w.is_contiguous():
+        raise ValueError(f"norm weights are BF16 vectors of head_dim values on cuda:{device}")
     return w.data_ptr()
 
 
@@ -117,26 +122,33 @@ class AttentionKernels:
             raise ValueError(f"the current device is not cuda:{self._device}, which these kernels were made for")
         return torch._C._cuda_getCurrentRawStream(self._device) if stream is None else stream.cuda_stream
 
+    def _here(self, *parts) -> int:
+        """The kernels' device, after a check that caches, sequences and rotations are there too."""
+        for p in parts:
+            if p is not None and p.device_index != self._device:
+                raise ValueError(f"{type(p).__name__} on device {p.device_index}, wanted cuda:{self._device}")
+        return self._device
+
     def qk_norm_rope(self, q, k, positions, rotary=None, q_weight=None, k_weight=None, eps=1e-6, q_out=None, k_out=None, stream=None):
         """Per-head RMS norm (where a weight is given) and rotation of q and k (k may be None); returns (q_out, k_out)."""
         rows, q_heads, dim = q.shape
-        dtype = q.dtype
+        dtype, at = q.dtype, self._here(rotary)
         if q_out is None:
             q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
         if positions is not None:
-            _need(positions.dtype is torch.int32 and positions.numel() == rows and positions.is_contiguous(), "positions: int32 [rows]")
+            _need(positions.dtype is torch.int32 and positions.numel() == rows and positions.is_contiguous() and positions.get_device() == at, "positions: int32 [rows] on the kernels' device")
         if k is not None:
             if k_out is None:
                 k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
             k_heads = k.shape[1]
             _need(k_out.shape[1] == k_heads, "k_out has as many heads as k")
-            k_args = (k.data_ptr(), k_out.data_ptr(), _row_stride(k, rows, dim, dtype, "k"), _row_stride(k_out, rows, dim, dtype, "k_out"), k_heads)
+            k_args = (k.data_ptr(), k_out.data_ptr(), _row_stride(k, rows, dim, dtype, "k", at), _row_stride(k_out, rows, dim, dtype, "k_out", at), k_heads)
         else:
             k_args = (None, None, 0, 0, 0)
         status = self.lib.padra_qk_norm_rope(
-            q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(q_out, rows, dim, dtype, "q_out"), q_heads, *k_args,
-            _weight(q_weight, dim), _weight(k_weight, dim), eps, None if positions is None else positions.data_ptr(), rotary and rotary.ref, rows, dim,
+            q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(q_out, rows, dim, dtype, "q_out", at), q_heads, *k_args,
+            _weight(q_weight, dim, at), _weight(k_weight, dim, at), eps, None if positions is None else positions.data_ptr(), rotary and rotary.ref, rows, dim,
             ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
         if status:
             raise B.PadraError(status, "padra_qk_norm_rope")
@@ -144,27 +156,27 @@ class AttentionKernels:
 
     def append(self, cache, sequences, k, v, rotary=None, k_weight=None, eps=1e-6, q=None, q_weight=None, q_out=None, stream=None):
         """Appends the rows' K (normed, rotated) and V; with q also norms and rotates the rows' queries and returns them."""
-        rows, dim, dtype = sequences.rows, cache.head_dim, k.dtype
+        rows, dim, dtype, at = sequences.rows, cache.head_dim, k.dtype, self._here(cache, sequences, rotary)
         _need(k.shape[1] == cache.kv_heads and v.shape[1] == cache.kv_heads, "k and v have the cache's heads")
         if q is not None:
             if q_out is None:
                 q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             q_heads = q.shape[1]
             _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
-            q_args = (q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(q_out, rows, dim, dtype, "q_out"), q_heads,
-                      _weight(q_weight, dim))
+            q_args = (q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(q_out, rows, dim, dtype, "q_out", at), q_heads,
+                      _weight(q_weight, dim, at))
         else:
             q_args = (None, None, 0, 0, 0, None)
         status = self.lib.padra_kv_append(
-            cache.ref, sequences.ref, k.data_ptr(), v.data_ptr(), _row_stride(k, rows, dim, dtype, "k"), _row_stride(v, rows, dim, dtype, "v"),
-            _weight(k_weight, dim), eps, rotary and rotary.ref, *q_args, ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
+            cache.ref, sequences.ref, k.data_ptr(), v.data_ptr(), _row_stride(k, rows, dim, dtype, "k", at), _row_stride(v, rows, dim, dtype, "v", at),
+            _weight(k_weight, dim, at), eps, rotary and rotary.ref, *q_args, ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
         if status:
             raise B.PadraError(status, "padra_kv_append")
         return q_out
 
     def read(self, cache, sequences, k_out=None, v_out=None, dtype=torch.bfloat16, stream=None):
         """The values of the cached tokens at the rows' positions; returns (k_out, v_out)."""
-        rows, heads, dim = sequences.rows, cache.kv_heads, cache.head_dim
+        rows, heads, dim, at = sequences.rows, cache.kv_heads, cache.head_dim, self._here(cache, sequences)
         if k_out is None:
             k_out = torch.empty((rows, heads, dim), dtype=dtype, device=cache.pool.device)
         if v_out is None:
@@ -172,8 +184,8 @@ class AttentionKernels:
         dtype = k_out.dtype
         _need(k_out.shape[1] == heads and v_out.shape[1] == heads, "k_out and v_out have the cache's heads")
         status = self.lib.padra_kv_read(
-            cache.ref, sequences.ref, k_out.data_ptr(), v_out.data_ptr(), _row_stride(k_out, rows, dim, dtype, "k_out"),
-            _row_stride(v_out, rows, dim, dtype, "v_out"), ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
+            cache.ref, sequences.ref, k_out.data_ptr(), v_out.data_ptr(), _row_stride(k_out, rows, dim, dtype, "k_out", at),
+            _row_stride(v_out, rows, dim, dtype, "v_out", at), ROWS_TYPE.get(dtype, -1), self._bad, self._stream(stream))
         if status:
             raise B.PadraError(status, "padra_kv_read")
         return k_out, v_out
@@ -192,13 +204,13 @@ class AttentionKernels:
 
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
         """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
-        rows, dim, dtype, heads = sequences.rows, cache.head_dim, q.dtype, q.shape[1]
+        rows, dim, dtype, heads, at = sequences.rows, cache.head_dim, q.dtype, q.shape[1], self._here(cache, sequences)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         _need(out.shape[1] == heads, "out has as many heads as q")
         stream = self._stream(stream)
         status = self.lib.padra_attention_q4(
-            cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _row_stride(q, rows, dim, dtype, "q"), _row_stride(out, rows, dim, dtype, "out"), heads,
+            cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(out, rows, dim, dtype, "out", at), heads,
             ROWS_TYPE.get(dtype, -1), scale, window, *self.workspace(dim, stream), self._bad, stream)
         if status:
             raise B.PadraError(status, "padra_attention_q4")

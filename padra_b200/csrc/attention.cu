@@ -30,7 +30,7 @@ namespace {
 using namespace attention;
 
 // Small CTAs, as many to an SM as the registers of a column block leave room for: what a CTA does between two pieces
-// (queries, joining its warps, tickets) runs under the others' tiles.
+// (queries, joining its warps) runs under the others' tiles.
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 template <int NT> struct Cta {
   static constexpr int kPerSm = NT == 1 ? 3 : 2;
@@ -234,6 +234,13 @@ template <typename T, int D, int NT> struct Piece {
       const unsigned tile = ring_address + (i & (kStages - 1)) * TileBytes<D>::kAll;
       const int t0 = (first_tile + warp + i * kWarps) * kTile;
       const bool edge = t0 + kTile - 1 > least || t0 < latest_low;
+      if (t0 < visible_low) { // tokens before every row's window may hold anything: a weight of zero does not make a NaN vanish
+        if (t0 + lane < visible_low)
+          for (int which = 0; which < 2; ++which)
+            for (int x = 0; x < D / 16; x += 4)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(tile + which * (TileBytes<D>::kCodes + TileBytes<D>::kScales) + TileBytes<D>::kCodes + lane * (D / 16) + x), "r"(0) : "memory");
+        __syncwarp();
+      }
 
       float score[2][NT][4];
 #pragma unroll

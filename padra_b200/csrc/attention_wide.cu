@@ -263,8 +263,9 @@ template <int D> struct Producer {
     else
       return (lane >> 4) * 8 + ((lane >> 3) & 1) * 2 + ((lane >> 1) & 1) + ((lane >> 2) & 1) * 4;
   }
-  // Codes and scales of this warp's 16 tokens from token t on; zeros (scale 0) for tokens at and beyond `context` or without a page.
-  __device__ __forceinline__ void Load(const AttentionArgs &a, int page, int head, int t, int context) {
+  // Codes and scales of this warp's 16 tokens from token t on; zeros (scale 0) for tokens outside [low, context) or without a page:
+  // their slots may hold anything, and a weight of zero does not make a NaN vanish.
+  __device__ __forceinline__ void Load(const AttentionArgs &a, int page, int head, int t, int low, int context) {
     const int lane = threadIdx.x & 31, chunk = lane % kChunks;
     const unsigned char *const block = a.cache.block(max(page, 0), head);
     const int slot = t & (a.cache.page_size - 1), code_bytes = a.cache.code_bytes(), both = code_bytes + a.cache.scale_bytes();
@@ -272,7 +273,7 @@ template <int D> struct Producer {
     for (int i = 0; i < kTokens; ++i) {
       const int token = TokenOf(lane, i);
       k[i] = v[i] = make_uint4(0, 0, 0, 0), k_scale[i] = v_scale[i] = make_uint2(0, 0);
-      if (page >= 0 && t + token < context) {
+      if (page >= 0 && t + token < context && t + token >= low) {
         const unsigned char *const codes = block + (slot + token) * (D / 2) + 16 * chunk, *const scales = block + code_bytes + (slot + token) * (D / 16);
         k[i] = __ldg(reinterpret_cast<const uint4 *>(codes)), v[i] = __ldg(reinterpret_cast<const uint4 *>(codes + both));
         if constexpr (kGroups == 4) {
@@ -478,14 +479,14 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     using P = Producer<D>;
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
     const int mine = 16 * (warp - kSoftmaxWarps), chunk = lane % P::kChunks; // this warp's tokens of a tile
-    int tile = 0, page = -1; // of the piece: the tile that is loaded next, and the page of the warp's tokens in it
+    int tile = 0, page = -1, low = 0; // of the piece: the tile that is loaded next, the page of the warp's tokens in it, the first token seen
     P data;
     auto find = [&]() {
       page = -1;
       if (walk.More()) {
         const int t = (walk.unit.first + walk.skip + tile) * kTile + mine;
         // first token that some column of the unit sees
-        const int low = a.window ? max(0, walk.rows.context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
+        low = a.window ? max(0, walk.rows.context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
         if (t < walk.rows.context && t + 16 > low)
           page = PageOf(a.seq, a.cache, walk.s, t, a.bad);
       }
@@ -507,7 +508,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     };
     auto load = [&]() { // that tile's codes, then the page of the one after it
       if (walk.More()) {
-        data.Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, walk.rows.context);
+        data.Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, low, walk.rows.context);
         if (++tile == walk.count)
           next_piece(), tile = 0;
         find();

@@ -418,3 +418,199 @@ def test_a_pool_of_more_than_four_gigabytes(gpu):
     want = R.dequantise(*R.quantise(c.k.double()))
     assert torch.equal(back.cpu().double(), want)
     assert not pool[:c.pool.shape[0]].any() and c.kernels.bad_flag() == 0
+
+
+def unwritten(c, window):
+    """Gives every slot that no row attends to scales that are NaN or infinite (all of K's and V's), on both sides."""
+    a, b = c.page * c.dim // 2, c.page * c.dim // 16
+    seen = torch.zeros((c.pool.shape[0], c.page), dtype=torch.bool)
+    for s, (n, ctx) in enumerate(c.shapes):
+        for t in range(max(0, ctx - n - window + 1) if window else 0, ctx if n else 0):
+            seen[int(c.table[s, t // c.page]), t % c.page] = True
+    for at in (a, 2 * a + b):
+        scales = c.pool[:, :, at:at + b].contiguous().view(torch.float16).view(c.pool.shape[0], c.kv_heads, c.page, c.dim // 32)
+        scales[~seen[:, None, :].expand(-1, c.kv_heads, -1)] = torch.tensor([float("nan"), float("inf")] * (c.dim // 64), dtype=torch.float16)
+        c.pool[:, :, at:at + b] = scales.view(torch.uint8).view(c.pool.shape[0], c.kv_heads, b)
+    c.cache.pool.copy_(c.pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(8, 2, 128, 64), (12, 1, 64, 16), (4, 4, 128, 256)])
+@pytest.mark.parametrize("shapes", [[(1, 200), (1, 1), (1, 77)], [(3, 150), (2, 19)], [(70, 200), (5, 131), (130, 130)], [(0, 90), (1, 0), (2, 1)]])
+@pytest.mark.parametrize("window", [0, 1, 20])
+def test_slots_that_nobody_attends_to_may_hold_anything(gpu, heads, kv_heads, dim, page, shapes, window):
+    c = Call(gpu, shapes, heads, kv_heads, dim, page, torch.bfloat16, 41, spare_rows=1)
+    unwritten(c, window)
+    live = c.reference
+
+    def reference(scale, window, pool=None):  # 0 * NaN stays out of the reference too
+        held = c.pool
+        c.pool = held.clone()
+        a, b = c.page * c.dim // 2, c.page * c.dim // 16
+        for at in (a, 2 * a + b):
+            s = c.pool[:, :, at:at + b].contiguous().view(torch.float16)
+            c.pool[:, :, at:at + b] = s.nan_to_num(0, 0, 0).view(torch.uint8)
+        try:
+            return live(scale, window)
+        finally:
+            c.pool = held
+
+    c.reference = reference
+    c.check_attention(window=window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads, rows, context", [
+    (8, 8, 1, 40000), (8, 2, 1, 40000), (16, 1, 1, 40000), (24, 1, 1, 20000), (300, 1, 1, 5000), (300, 1, 7, 600), (8, 2, 2, 9001), (8, 1, 5, 9001),
+    (8, 8, 9, 5000), (16, 1, 33, 2100), (8, 2, 300, 2500), (4, 1, 130, 6000)])
+def test_one_sequence_split_over_the_gpu(gpu, heads, kv_heads, rows, context):
+    """Many pieces of one unit: few and many joins, one, several and many blocks of columns."""
+    Call(gpu, [(rows, context)], heads, kv_heads, 64, 64, torch.bfloat16, 43).check_attention(window=0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count, most_rows", [(1, 1), (33, 2), (129, 1), (700, 1), (700, 5), (150, 40)])
+def test_many_sequences(gpu, count, most_rows):
+    g = torch.Generator().manual_seed(count)
+    shapes = []
+    for _ in range(count):
+        n = int(torch.randint(0, most_rows + 1, (1,), generator=g))
+        shapes.append((n, n + int(torch.randint(0, 90, (1,), generator=g))))
+    c = Call(gpu, shapes, 4, 2, 64, 16, torch.bfloat16, 47, spare_rows=3)
+    c.check_attention()
+    c.check_attention(window=9)
+    q = c.kernels.append(c.cache, c.sequences, c.dk, c.dv, q=c.dq, q_out=torch.zeros_like(c.dq))
+    k, v = c.kernels.read(c.cache, c.sequences, torch.zeros_like(c.dk, dtype=torch.float32), torch.zeros_like(c.dv, dtype=torch.float32))
+    last = int(c.begin[-1])
+    for x, got in ((c.k, k), (c.v, v)):
+        assert torch.equal(got[:last].cpu().double(), R.dequantise(*R.quantise(x[:last].double())))
+    assert torch.equal(q[:last], c.dq[:last]) and not q[last:].any() and not k[last:].any() and c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 3, 20, 130])
+@pytest.mark.parametrize("order", [1, -1])
+def test_scores_that_rise_and_fall_along_the_axis(gpu, rows, order):
+    """Scores from -100 to 100: the running maximum moves with every tile, or never after the first."""
+    c = Call(gpu, [(rows, 1500)], 4, 2, 64, 32, torch.float16, 53)
+    c.q[:] = 0.25
+    c.d_qkv.copy_(c.qkv)
+    for t in range(1500):
+        k = torch.full((64,), order * (t - 750) / 750, dtype=torch.float64)
+        for h in range(2):
+            R.store(c.pool, int(c.table[0, t // 32]), h, t % 32, 32, k, torch.full((64,), float(t % 50), dtype=torch.float64))
+    c.cache.pool.copy_(c.pool)
+    c.check_attention(scale=6.25)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(1, 3000)] * 3, [(5, 900), (2, 17)], [(100, 700), (30, 2000)]])
+def test_calls_repeat_bit_for_bit_whatever_the_workspace_held(gpu, shapes):
+    c = Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 59)
+    first = c.check_attention()
+    stream = torch.cuda.current_stream().cuda_stream
+    for fill in (255, 0, 127):
+        c.kernels._workspace[stream, 128][2].fill_(fill)
+        assert torch.equal(c.kernels.attention(c.cache, c.sequences, c.dq, 128 ** -0.5), first)
+
+
+@pytest.mark.gpu
+def test_pages_shared_by_sequences_that_only_read_them(gpu):
+    c = Call(gpu, [(1, 64), (1, 64), (20, 64)], 4, 2, 64, 16, torch.bfloat16, 61)
+    for s in (1, 2):  # the first three pages of all are the first sequence's
+        c.table[s, :3] = c.table[0, :3]
+    c.sequences.page_table.copy_(c.table)
+    c.check_attention()
+
+
+@pytest.mark.gpu
+def test_two_streams_and_a_captured_call(gpu):
+    calls = [Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 67 + i) for i, shapes in enumerate(([(1, 5000), (1, 300)], [(40, 900), (3, 100)]))]
+    kernels = calls[0].kernels
+    alone = [kernels.attention(c.cache, c.sequences, c.dq, 0.1) for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):  # side by side, each stream with its own workspace
+        for c, stream, out in zip(calls, streams, outs):
+            with torch.cuda.stream(stream):
+                out.append(kernels.attention(c.cache, c.sequences, c.dq, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for out, want in zip(outs, alone) for x in out)
+    # a captured append + attention, replayed with new rows, another page table and another context
+    c = calls[0]
+    out, q = torch.zeros_like(c.dq, memory_format=torch.contiguous_format), torch.zeros_like(c.dq, memory_format=torch.contiguous_format)
+
+    def step():
+        kernels.append(c.cache, c.sequences, c.dk, c.dv, q=c.dq, q_out=q)
+        kernels.attention(c.cache, c.sequences, q, 0.1, out=out)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[0]):
+        step()
+    pool = c.cache.pool.clone()
+    for context in ([5000, 300], [4097, 0], [1, 320]):
+        c.sequences.context.copy_(torch.tensor(context, dtype=torch.int32))
+        if context[1] == 320:
+            c.sequences.page_table.copy_(torch.randint(0, c.pool.shape[0], c.table.shape, generator=c.g))
+            c.sequences.page_table[1, 4] = (c.sequences.page_table[0, 0] + 1) % c.pool.shape[0]  # appended to by one sequence only
+        c.d_qkv.copy_(torch.randn(c.qkv.shape, generator=c.g))
+        c.cache.pool.copy_(pool)
+        graph.replay()
+        got, after = out.clone(), c.cache.pool.clone()
+        c.cache.pool.copy_(pool)
+        step()
+        assert torch.equal(out, got) and torch.equal(c.cache.pool, after) and kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+def test_a_workspace_is_not_made_under_capture(gpu):
+    c = Call(gpu, [(1, 20)], 4, 2, 64, 16, torch.bfloat16, 71)
+    stream = torch.cuda.Stream()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):
+        with pytest.raises(ValueError, match="workspace"):
+            c.kernels.attention(c.cache, c.sequences, c.dq, 0.1)
+
+
+@pytest.mark.gpu
+def test_tensors_elsewhere_and_other_layouts_are_refused(gpu):
+    c = Call(gpu, [(2, 20)], 4, 2, 64, 16, torch.bfloat16, 73)
+    k, call = c.kernels, (c.cache, c.sequences)
+    with pytest.raises(ValueError):  # on the CPU
+        k.attention(*call, c.q, 0.1)
+    with pytest.raises(ValueError):
+        k.append(*call, c.k, c.v)
+    with pytest.raises(ValueError):
+        k.append(*call, c.dk, c.dv, q=c.dq, q_weight=torch.ones(64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        k.qk_norm_rope(c.q, None, None)
+    from padra_b200 import attention as A
+
+    with pytest.raises(ValueError):
+        k.attention(A.KvCache.over(c.pool, 16, 64), c.sequences, c.dq, 0.1)
+    with pytest.raises(ValueError):
+        k.read(c.cache, A.Sequences(c.table, c.begin, c.context, c.rows, 2))
+    with pytest.raises(ValueError):
+        k.append(*call, c.dk, c.dv, A.Rotary(torch.zeros(32, dtype=torch.float64)))
+    with pytest.raises(ValueError):  # heads apart
+        k.attention(*call, c.d_qkv[:, :8 * 64].unflatten(1, (8, 64))[:, ::2], 0.1)
+    with pytest.raises(ValueError):
+        k.attention(*call, c.dq.transpose(1, 2).contiguous().transpose(1, 2), 0.1)
+    with pytest.raises(ValueError):
+        k.attention(*call, c.dq[:1], 0.1)
+    with pytest.raises(A.B.PadraError):  # seven heads over two
+        k.attention(*call, torch.zeros((2, 7, 64), dtype=torch.bfloat16, device=gpu), 0.1)
+    with pytest.raises(A.B.PadraError):
+        k.attention(*call, c.dq.float(), 0.1)
+    assert k.bad_flag() == 0
+
+
+@pytest.mark.gpu
+def test_a_flag_that_is_up_changes_nothing(gpu):
+    c = Call(gpu, [(1, 700), (30, 100)], 4, 2, 64, 16, torch.bfloat16, 79)
+    want = c.check_attention()
+    c.kernels.bad.fill_(1)
+    assert torch.equal(c.kernels.attention(c.cache, c.sequences, c.dq, 64 ** -0.5), want)
+    c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
+    k, _ = c.kernels.read(c.cache, c.sequences, dtype=torch.float32)
+    assert torch.equal(k.cpu().double(), R.dequantise(*R.quantise(c.k.double()))) and c.kernels.bad_flag() == 1
