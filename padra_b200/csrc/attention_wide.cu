@@ -265,22 +265,22 @@ template <int D> struct Producer {
   }
   // Codes and scales of this warp's 16 tokens from token t on; zeros (scale 0) for tokens outside [low, context) or without a page:
   // their slots may hold anything, and a weight of zero does not make a NaN vanish.
-  __device__ __forceinline__ void Load(const AttentionArgs &a, int page, int head, int t, int low, int context) {
+  static __device__ __forceinline__ void Load(const AttentionArgs &a, int page, int head, int t, int low, int context, int offset, uint4 (&words)[kTokens],
+                                              uint2 (&scale)[kTokens]) { // offset: of K or V in the block
     const int lane = threadIdx.x & 31, chunk = lane % kChunks;
-    const unsigned char *const block = a.cache.block(max(page, 0), head);
-    const int slot = t & (a.cache.page_size - 1), code_bytes = a.cache.code_bytes(), both = code_bytes + a.cache.scale_bytes();
+    const unsigned char *const block = a.cache.block(max(page, 0), head) + offset;
+    const int slot = t & (a.cache.page_size - 1), code_bytes = a.cache.code_bytes();
 #pragma unroll
     for (int i = 0; i < kTokens; ++i) {
       const int token = TokenOf(lane, i);
-      k[i] = v[i] = make_uint4(0, 0, 0, 0), k_scale[i] = v_scale[i] = make_uint2(0, 0);
+      words[i] = make_uint4(0, 0, 0, 0), scale[i] = make_uint2(0, 0);
       if (page >= 0 && t + token < context && t + token >= low) {
         const unsigned char *const codes = block + (slot + token) * (D / 2) + 16 * chunk, *const scales = block + code_bytes + (slot + token) * (D / 16);
-        k[i] = __ldg(reinterpret_cast<const uint4 *>(codes)), v[i] = __ldg(reinterpret_cast<const uint4 *>(codes + both));
-        if constexpr (kGroups == 4) {
-          k_scale[i] = __ldg(reinterpret_cast<const uint2 *>(scales)), v_scale[i] = __ldg(reinterpret_cast<const uint2 *>(scales + both));
-        } else {
-          k_scale[i].x = __ldg(reinterpret_cast<const unsigned *>(scales)), v_scale[i].x = __ldg(reinterpret_cast<const unsigned *>(scales + both));
-        }
+        words[i] = __ldg(reinterpret_cast<const uint4 *>(codes));
+        if constexpr (kGroups == 4)
+          scale[i] = __ldg(reinterpret_cast<const uint2 *>(scales));
+        else
+          scale[i].x = __ldg(reinterpret_cast<const unsigned *>(scales));
       }
     }
   }
@@ -481,14 +481,16 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
     const int mine = 16 * (warp - kSoftmaxWarps), chunk = lane % P::kChunks; // this warp's tokens of a tile
     int tile = 0, page = -1, low = 0; // of the piece: the tile that is loaded next, the page of the warp's tokens in it, the first token seen
     P data;
-    auto find = [&]() {
+    auto find = [&]() { // the page is checked only when it is used: its load takes as long as the codes'
       page = -1;
       if (walk.More()) {
         const int t = (walk.unit.first + walk.skip + tile) * kTile + mine;
         // first token that some column of the unit sees
         low = a.window ? max(0, walk.rows.context - walk.rows.rows + walk.block * kColumns / a.group + 1 - a.window) : 0;
         if (t < walk.rows.context && t + 16 > low)
-          page = PageOf(a.seq, a.cache, walk.s, t, a.bad);
+          page = __ldg(a.seq.page_table + static_cast<long long>(walk.s) * a.seq.table_stride + (t >> a.cache.page_shift));
+        else
+          low = 0x7fffffff; // no token of the warp counts
       }
     };
     // A piece's queries come before its first tile: this warp's 32 columns, once the MMAs of the piece before are done with Q.
@@ -506,19 +508,24 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       }
       ++pieces;
     };
-    auto load = [&]() { // that tile's codes, then the page of the one after it
-      if (walk.More()) {
-        data.Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, low, walk.rows.context);
-        if (++tile == walk.count)
-          next_piece(), tile = 0;
-        find();
-      }
+    auto load_k = [&]() {
+      if (low != 0x7fffffff && (page < 0 || page >= a.cache.pages))
+        Raise(a.bad), page = -1;
+      P::Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, low, walk.rows.context, 0, data.k, data.k_scale);
+    };
+    auto load_v = [&]() { // then the page of the tile after it
+      P::Load(a, page, walk.head, (walk.unit.first + walk.skip + tile) * kTile + mine, low, walk.rows.context, a.cache.code_bytes() + a.cache.scale_bytes(),
+              data.v, data.v_scale);
+      if (++tile == walk.count)
+        next_piece(), tile = 0;
+      find();
     };
     bool have = walk.More(); // a tile has been loaded and not been stored
     if (have) {
       find();
       stage_queries();
-      load();
+      load_k();
+      load_v();
     }
     for (unsigned n = 0; have && alive; ++n) {
       const int stage = n & (kStages - 1);
@@ -533,6 +540,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       __syncwarp();
       if (lane == 0)
         BarrierArrive(&sm.k_full[stage]);
+      have = walk.More();
+      if (have)
+        load_k(); // the next tile's keys come while this one's values are converted, its values while its keys are
       alive = WarpWait(&sm.v_empty[stage], free_parity, abort);
       if (!alive)
         break;
@@ -543,11 +553,10 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       __syncwarp();
       if (lane == 0)
         BarrierArrive(&sm.v_full[stage]);
-      have = walk.More();
       if (have) {
         if (tile == 0) // the next tile begins a piece
           stage_queries();
-        load(); // arrives while the MMAs free the next stage
+        load_v();
       }
     }
   } else if (warp >= kMmaWarp) {
