@@ -16,6 +16,8 @@
 //     each with its own maximum, sum and O, and are joined through tensor memory at the end of the piece.
 // Tensor memory: S/P of the halves in columns 0 and 128, O in 256 and 384.  Every wait is bounded in time; on expiry the CTA raises the
 // error flag and leaves.
+#include <type_traits>
+
 #include "attention.cuh"
 
 namespace padra {
@@ -460,7 +462,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
   BeforeSync();
   __syncthreads();
   AfterSync();
-  const unsigned tmem = sm.tmem;
+  constexpr unsigned tmem = 0; // all 512 columns are this CTA's; addresses known to the compiler make an MMA some 10 instructions instead of 100
   const volatile int *const abort = &sm.abort;
   Walk &walk = sm.walk[min(warp, kMmaWarp)];
   if (lane == 0 && warp <= kMmaWarp)
@@ -472,7 +474,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       walk.Next(a);
     __syncwarp();
   };
-  bool alive = true;
+  bool alive = sm.tmem == 0;
 
   if (warp >= kSoftmaxWarps && warp < kMmaWarp) {
     // =============================== producers ===============================
@@ -569,8 +571,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       for (; alive && walk.More(); walk.Next(a)) {
         const bool paired = walk.Paired();
         const int jobs = paired ? walk.count : 2 * walk.count;
-        auto scores = [&](int i) { // S of job i
-          const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
+        auto scores = [&](int i, auto half) { // S of job i
+          const int tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
           if (paired || half == 0)
             if (!(alive = SuspendedWait(&sm.k_full[stage], ((tiles + tile) / kStages) & 1, abort)))
               return;
@@ -587,21 +589,13 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           if (i == jobs - 1)
             MmaCommit(&sm.q_empty);
         };
-        // Q of this piece: the second half's tile is staged only where it has columns of its own
-        alive = SuspendedWait(&sm.q_full[0], pieces_of[0]++ & 1, abort);
-        if (alive)
-          scores(0);
-        if (alive && !paired)
-          alive = SuspendedWait(&sm.q_full[1], pieces_of[1]++ & 1, abort);
-        if (alive && jobs > 1)
-          scores(1);
-        for (int i = 0; i < jobs && alive; ++i) {
-          const int half = i & 1, tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
+        auto outputs = [&](int i, auto half) { // O += P V of job i, then S of the job after the next
+          const int tile = paired ? i : i >> 1, stage = (tiles + tile) & (kStages - 1);
           if (paired || half == 0)
             if (!(alive = SuspendedWait(&sm.v_full[stage], ((tiles + tile) / kStages) & 1, abort)))
-              break;
+              return;
           if (!(alive = SuspendedWait(&sm.p_full[half], jobs_of[half]++ & 1, abort)))
-            break;
+            return;
           AfterSync();
           const unsigned v_low = DescriptorLow(SmemAddress(sm.v[stage][0]), 128 * 128);
 #pragma unroll
@@ -612,7 +606,22 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           if (i + 2 >= jobs)
             MmaCommit(&sm.o_full[half]);
           else
-            scores(i + 2);
+            scores(i + 2, half);
+        };
+        constexpr std::integral_constant<int, 0> kFirst{};
+        constexpr std::integral_constant<int, 1> kSecond{};
+        // Q of this piece: the second half's tile is staged only where it has columns of its own
+        alive = SuspendedWait(&sm.q_full[0], pieces_of[0]++ & 1, abort);
+        if (alive)
+          scores(0, kFirst);
+        if (alive && !paired)
+          alive = SuspendedWait(&sm.q_full[1], pieces_of[1]++ & 1, abort);
+        if (alive && jobs > 1)
+          scores(1, kSecond);
+        for (int i = 0; i < jobs && alive; i += 2) {
+          outputs(i, kFirst);
+          if (alive && i + 1 < jobs)
+            outputs(i + 1, kSecond);
         }
         tiles += walk.count;
       }
@@ -829,7 +838,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       __nanosleep(1000);
   if (warp == kMmaWarp) {
     AfterSync();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem), "r"(512) : "memory");
   }
 }
 
