@@ -678,40 +678,54 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           }
           TmemStoreWait();
         }
-        float most = -INFINITY;
-#pragma unroll 1
-        for (int piece = 0; piece < 2; ++piece) {
-          float x[64];
-          TmemLoad64(s_address + 64 * piece, x);
-          float part[2] = {most, x[0]};
-#pragma unroll
-          for (int j = 0; j < 64; j += 2)
-            part[j >> 1 & 1] = Max3(part[j >> 1 & 1], x[j], x[j + 1]);
-          most = fmaxf(part[0], part[1]);
-        }
-        const bool raise = fmaf(most, factor, -top) > kRaise;
-        if (__any_sync(0xffffffffu, raise)) {
-          const float next = raise ? fmaf(most, factor, -kTop) : top, shrink = Exp2(top - next);
-          top = next, total *= shrink;
-          if (i != begin_tile) { // the S that has just come says that the MMAs before it are done with O
-#pragma unroll 1
-            for (int piece = 0; piece < D / 16; ++piece) {
-              float y[16];
-              TmemLoad16(o_address + 16 * piece, y);
-              unsigned z[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j)
-                z[j] = __float_as_uint(y[j] * shrink);
-              TmemStore16(o_address + 16 * piece, z);
-            }
-          }
-        }
-        const float2 factors = make_float2(factor, factor), minus_top = make_float2(-top, -top);
+        // 64 scores at a time, from tensor memory once: a maximum that is raised in the second half of the tile scales the first's weights too
         float2 sum[2] = {make_float2(total, 0), make_float2(0, 0)};
 #pragma unroll 1
         for (int piece = 0; piece < 2; ++piece) {
           float x[64];
           TmemLoad64(s_address + 64 * piece, x);
+          float part[2] = {x[0], x[1]};
+#pragma unroll
+          for (int j = 2; j < 64; j += 2)
+            part[j >> 1 & 1] = Max3(part[j >> 1 & 1], x[j], x[j + 1]);
+          const float most = fmaxf(part[0], part[1]);
+          const bool raise = fmaf(most, factor, -top) > kRaise;
+          if (__any_sync(0xffffffffu, raise)) {
+            const float next = raise ? fmaf(most, factor, -kTop) : top, shrink = Exp2(top - next);
+            top = next;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              sum[k].x *= shrink, sum[k].y *= shrink;
+            if (piece) {
+              TmemStoreWait();
+#pragma unroll 1
+              for (int k = 0; k < 32; k += 16) {
+                float y[16];
+                TmemLoad16(s_address + k, y);
+                unsigned z[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                  const __half2 p = __hmul2(*reinterpret_cast<const __half2 *>(&y[j]), __float2half2_rn(shrink));
+                  z[j] = *reinterpret_cast<const unsigned *>(&p);
+                }
+                TmemStore16(s_address + k, z);
+              }
+            }
+            if (i != begin_tile) { // the S that has just come says that the MMAs before it are done with O
+#pragma unroll 1
+              for (int k = 0; k < D / 16; ++k) {
+                float y[16];
+                TmemLoad16(o_address + 16 * k, y);
+                unsigned z[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                  z[j] = __float_as_uint(y[j] * shrink);
+                TmemStore16(o_address + 16 * k, z);
+              }
+            }
+            TmemLoad64(s_address + 64 * piece, x); // again: not held over all this
+          }
+          const float2 factors = make_float2(factor, factor), minus_top = make_float2(-top, -top);
           unsigned packed[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
