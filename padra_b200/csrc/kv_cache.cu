@@ -323,9 +323,20 @@ __device__ __forceinline__ void NormRotateKey(double (&x)[8], int at, const unsi
   }
 }
 
+// Adding and subtracting kInteger rounds to an integer, which is then in the sum's low bits.
+template <typename Real> struct Rounding;
+template <> struct Rounding<float> {
+  static constexpr float kInteger = 12582912.f; // 1.5 * 2^23
+  static __device__ __forceinline__ unsigned LowBits(float x) { return __float_as_uint(x) - 0x4b400000u; }
+};
+template <> struct Rounding<double> {
+  static constexpr double kInteger = 6755399441055744.0; // 1.5 * 2^52
+  static __device__ __forceinline__ unsigned LowBits(double x) { return static_cast<unsigned>(__double2loint(x)); }
+};
+
 // Eight values of a lane as eight codes, four lanes to a group.  The code is the nearest of x / scale, ties to even, as a division in 64
-// bits would give it, without the division: a guess in 32 bits is off by one at most (its error is far below one half), and
-// what is left of x, exact or rounded far below the difference between two inputs, decides.
+// bits would give it, without the division: a product with 1 / scale in 32 bits (its error is far below one half) gives an integer, and
+// what is left of x, exact or rounded far below the difference between two inputs, tells whether that is the nearest one.
 template <typename Real> __device__ __forceinline__ unsigned QuantiseWord(const Real (&x)[8], unsigned short *scale_bits, bool *fine) {
   Real most = 0;
   bool finite = true;
@@ -340,18 +351,27 @@ template <typename Real> __device__ __forceinline__ unsigned QuantiseWord(const 
   *fine = finite && most <= static_cast<Real>(kKvLargest);
   const __half h = __double2half(static_cast<double>(most) / 7.0);
   const float scale = __half2float(h), inverse = scale > 0 ? 1.f / scale : 0.f;
-  const Real step = static_cast<Real>(scale), half = static_cast<Real>(0.5f * scale);
-  unsigned word = 0;
+  const Real step = static_cast<Real>(scale), half = static_cast<Real>(0.5f * scale), factor = static_cast<Real>(inverse);
+  Real worst = 0;
+  unsigned word = 0x88888888u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // a scale that was rounded down may leave 7.x steps, and one below FP16's normal range many more
-    const float guess = fminf(fmaxf(rintf(static_cast<float>(x[i]) * inverse), -8.f), 8.f);
-    const Real rest = fma(-static_cast<Real>(guess), step, x[i]);
-    int code = static_cast<int>(guess);
-    const bool odd = code & 1;
-    code += (rest > half || (rest == half && odd)) - (rest < -half || (rest == -half && odd));
-    code = scale > 0 ? min(max(code, -7), 7) : 0;
-    word |= static_cast<unsigned>(code + 8) << (4 * i);
+    const Real sum = fma(x[i], factor, Rounding<Real>::kInteger), guess = sum - Rounding<Real>::kInteger;
+    worst = max(worst, abs(fma(-guess, step, x[i])));
+    word += Rounding<Real>::LowBits(sum) << (4 * i);
+  }
+  // a tie, a guess that is off by one, or a scale below FP16's normal range, of which there may be more than seven steps
+  if (scale > 0 && (worst >= half || static_cast<float>(most) * inverse >= 7.5f)) {
+    word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float guess = fminf(fmaxf(rintf(static_cast<float>(x[i]) * inverse), -8.f), 8.f);
+      const Real rest = fma(-static_cast<Real>(guess), step, x[i]);
+      int code = static_cast<int>(guess);
+      const bool odd = code & 1;
+      code += (rest > half || (rest == half && odd)) - (rest < -half || (rest == -half && odd));
+      word |= static_cast<unsigned>(min(max(code, -7), 7) + 8) << (4 * i);
+    }
   }
   *scale_bits = __half_as_ushort(h);
   return word;
