@@ -373,7 +373,8 @@ PADRA_API int padra_qk_norm_rope(const void *q, void *q_out, long long q_stride,
                                  const int *positions, const padra_rotary *rotary, int rows, int head_dim, int type,
                                  int *bad, padra_stream stream);
 /* Appends the rows' K (normed with k_weight unless NULL, rotated unless rotary is NULL) and V to the cache, and, when q is
- * given, writes the rows' normed and rotated Q to q_out in the same launch.  K is normed and rotated in 64 bits and not
+ * given, writes the rows' normed and rotated Q to q_out in the same launch (padra_qk_norm_rope's values, which may
+ * differ in the last bit).  K is normed and rotated in 64 bits and not
  * rounded before it becomes codes, so the cache's bytes depend on the inputs alone and not on batch or launch shape.
  * A K or V head with a value that is not finite or above 57344 in magnitude (where FP16 values of the codes end) raises
  * *bad and is not written. */

@@ -614,3 +614,65 @@ def test_a_flag_that_is_up_changes_nothing(gpu):
     c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
     k, _ = c.kernels.read(c.cache, c.sequences, dtype=torch.float32)
     assert torch.equal(k.cpu().double(), R.dequantise(*R.quantise(c.k.double()))) and c.kernels.bad_flag() == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, heads, kv_heads, dim, interleaved", [(torch.bfloat16, 5, 3, 128, False), (torch.float32, 4, 2, 64, True), (torch.float16, 1, 1, 64, False)])
+def test_rows_do_not_depend_on_how_many_share_a_call(gpu, dtype, heads, kv_heads, dim, interleaved):
+    """One call for all rows against calls for 1, 40, 650 and the remaining rows: launch shapes differ, bytes do not."""
+    from padra_b200 import attention as A
+
+    total = 2900
+    c = Call(gpu, [(total, total + 7)], heads, kv_heads, dim, 64, dtype, 83)
+    weight = (1 + 0.3 * torch.randn(dim, generator=c.g)).bfloat16().to(gpu)
+    inv_freq, amplitude = R.yarn_like(dim // 2, 2.0)
+    rotary = A.Rotary(inv_freq.to(gpu), interleaved, amplitude)
+    before = c.cache.pool.clone()
+    q = c.kernels.append(c.cache, c.sequences, c.dk, c.dv, rotary, weight, 1e-6, c.dq, weight)
+    whole = c.cache.pool.clone()
+    positions = torch.arange(7, total + 7, dtype=torch.int32, device=gpu)
+    q_plain, k_plain = c.kernels.qk_norm_rope(c.dq, c.dk, positions, rotary, weight, weight)
+    read = c.kernels.read(c.cache, c.sequences, dtype=torch.float32)
+    c.cache.pool.copy_(before)
+    at = 0
+    for n in (1, 40, 650, total - 691):
+        part = slice(at, at + n)
+        begin = torch.tensor([0, n], dtype=torch.int32, device=gpu)
+        seq = A.Sequences(c.sequences.page_table, begin, torch.tensor([7 + at + n], dtype=torch.int32, device=gpu), n, n)
+        assert torch.equal(c.kernels.append(c.cache, seq, c.dk[part], c.dv[part], rotary, weight, 1e-6, c.dq[part], weight), q[part])
+        got = c.kernels.qk_norm_rope(c.dq[part], c.dk[part], positions[part], rotary, weight, weight)
+        assert torch.equal(got[0], q_plain[part]) and torch.equal(got[1], k_plain[part])
+        assert all(torch.equal(x, y[part]) for x, y in zip(c.kernels.read(c.cache, seq, dtype=torch.float32), read))
+        at += n
+    assert torch.equal(c.cache.pool, whole) and c.kernels.bad_flag() == 0
+    # the first and the last rows against the formulas
+    for r in (0, 1, 700, total - 1):
+        p = torch.tensor([r + 7])
+        want = R.rotate(R.rms(c.q[r:r + 1], weight.cpu(), 1e-6), p, inv_freq, interleaved, amplitude)
+        slack = 2.0 ** -19 * 2 * amplitude * want.abs().amax(-1, keepdim=True) * math.sqrt(2)
+        for got in (q, q_plain):  # either call rounds cos and sin its own way: near the same values, not the same bits
+            assert ((got[r:r + 1].cpu().double() - want).abs() <= HALF[dtype] * want.abs() + slack).all()
+        k = R.rotate(R.rms(c.k[r:r + 1], weight.cpu(), 1e-6), p, inv_freq, interleaved, amplitude)
+        assert torch.equal(read[0][r:r + 1].cpu().double(), R.dequantise(*R.quantise(k)))
+
+
+@pytest.mark.gpu
+def test_values_on_and_beside_the_borders_of_codes(gpu):
+    """Scales that are powers of two and others, values exactly between two codes and one step of FP32 to either side, scales below
+    FP16's normal range: the bytes of a division in 64 bits."""
+    rows = 64
+    c = Call(gpu, [(rows, rows)], 1, 2, 64, 16, torch.float32, 89)
+    g = torch.Generator().manual_seed(5)
+    for r in range(rows):
+        scale = 2.0 ** -(r % 27) * (1 if r % 2 else 1.1376953125)
+        x = (torch.randint(-7, 8, (4, 64), generator=g) + torch.tensor([0.5, -0.5, 0.0, 0.5])[:, None]).clamp(-7, 7) * scale
+        x[:, ::32] = 7 * scale
+        x = torch.where(torch.rand(x.shape, generator=g) < 0.3, torch.nextafter(x, x * 2), torch.where(torch.rand(x.shape, generator=g) < 0.3, torch.nextafter(x, x * 0), x))
+        c.k[r], c.v[r] = x[:2], x[2:]
+    c.d_qkv.copy_(c.qkv)
+    c.kernels.append(c.cache, c.sequences, c.dk, c.dv)
+    want = c.pool.clone()
+    for r in range(rows):
+        for h in range(2):
+            R.store(want, int(c.table[0, r // 16]), h, r % 16, 16, c.k[r, h].double(), c.v[r, h].double())
+    assert torch.equal(c.cache.pool.cpu(), want) and c.kernels.bad_flag() == 0

@@ -173,3 +173,24 @@ def test_refusals(gpu, layer):
             DecoderLayer(0, LayerWeights(**{**w, name: value}), layer.attention, layer.experts, layer.cache)
     empty = torch.zeros((0, HIDDEN), device=gpu)
     assert layer(empty, sequences(layer, [0, 0, 0], [5, 5, 5], 0)) is empty
+
+
+@pytest.mark.parametrize("rows", [17, 2050])
+def test_chunks_longer_than_one_schedule(gpu, layer, rows):
+    """2050 rows are a chunk of 2048 and a tail of two: every part as if it were alone."""
+    g = torch.Generator().manual_seed(rows)
+    normalized = torch.randn((rows, HIDDEN), generator=g).bfloat16().float().to(gpu)
+    x = torch.randn((rows, HIDDEN), generator=g).bfloat16().float().to(gpu)
+    got = x.clone()
+    layer.feed_forward(got, normalized)
+    logits = (normalized.bfloat16() @ layer.weights.router.T).float()
+    for at in range(0, rows, 2048):
+        n = min(2048, rows - at)
+        want, part = x[at:at + n].clone(), slice(at, at + n)
+        ids, routing = layer.experts.route(logits[part])
+        if n > 3:
+            layer.experts.prefill_layer(0, ids.reshape(-1), routing.reshape(-1), normalized[part].contiguous(), want, n)
+        else:
+            layer.experts.moe_decode_layer(0, ids, routing, normalized[part].contiguous(), want, n)
+        assert torch.equal(got[part], want)
+    assert layer.experts.bad_flag() == 0 and not torch.equal(got, x)
