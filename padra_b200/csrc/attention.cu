@@ -23,6 +23,7 @@
 // Measured: 64 sequences of 1 to 16384 tokens, 32 heads over 4, head size 128: 81 us, 3.8 TB/s of codes and scales (58% of a copy), bound by
 // instruction issue; one sequence of 131072 tokens: 24 us and 7 us for the join; of 4097: 13 us, all latency.
 #include <cmath>
+#include <type_traits>
 
 #include "attention.cuh"
 
@@ -76,6 +77,9 @@ template <int D> struct TileBytes {
 template <typename T, int D, int NT> struct Piece {
   static constexpr int kGroups = D / kKvGroup, kChunks = D / 32, kColumns = 8 * NT;
   static constexpr int kRow = D + 4; // floats of a column's row in shared memory while warps are joined
+  // FP16 rows are rounded by 2^-11 themselves, so that the weights' own rounding shows beside it: what it leaves off goes through a second
+  // MMA (error against 64 bits 0.00028 instead of 0.00033, the output's rounding alone 0.00021).  BF16 rows hide it.
+  static constexpr bool kRests = std::is_same<T, __half>::value;
 
   // column -> row of the sequence and head of the group
   static __device__ __forceinline__ void Run(const AttentionArgs &a, const Demand &d, int s, int head, int block, int first_tile, int count,
@@ -322,7 +326,7 @@ template <typename T, int D, int NT> struct Piece {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         // weights, transposed from (token, column) to (column, token)
-        unsigned p[NT][2];
+        unsigned p[NT][2], rest[kRests ? NT : 1][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -330,7 +334,12 @@ template <typename T, int D, int NT> struct Piece {
             const float p0 = Exp2(fmaf(score[half][n][2 * r], factor[n][0], -top[n][0])),
                         p1 = Exp2(fmaf(score[half][n][2 * r + 1], factor[n][1], -top[n][1]));
             sum[n][0] += p0, sum[n][1] += p1;
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][r]) : "r"(Pack(p0, p1)));
+            const unsigned weights = Pack(p0, p1);
+            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][r]) : "r"(weights));
+            if constexpr (kRests) {
+              const float2 rounded = __half22float2(*reinterpret_cast<const __half2 *>(&weights));
+              asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(rest[n][r]) : "r"(Pack(p0 - rounded.x, p1 - rounded.y)));
+            }
           }
         // V's scales of tokens 2c, 2c + 1 and 2c + 8, 2c + 9 in this lane's group
         const unsigned values = tile + TileBytes<D>::kCodes + TileBytes<D>::kScales;
@@ -360,6 +369,10 @@ template <typename T, int D, int NT> struct Piece {
             for (int n = 0; n < NT; ++n) {
               MmaF16(o[n][2 * (j + k)], a0, a1, a2, a3, p[n][0], p[n][1]);
               MmaF16(o[n][2 * (j + k) + 1], b0, b1, b2, b3, p[n][0], p[n][1]);
+              if constexpr (kRests) {
+                MmaF16(o[n][2 * (j + k)], a0, a1, a2, a3, rest[n][0], rest[n][1]);
+                MmaF16(o[n][2 * (j + k) + 1], b0, b1, b2, b3, rest[n][0], rest[n][1]);
+              }
             }
           }
         }
