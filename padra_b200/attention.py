@@ -93,6 +93,15 @@ def _row_stride(x: torch.Tensor, rows: int, dim: int, dtype: torch.dtype, what: 
     return stride[0]
 
 
+def _empty(shape, dtype: torch.dtype, device, stream) -> torch.Tensor:
+    """Memory for a call on `stream` (None: the current one): taken there, since work on the current stream may still be using what
+    the current stream has given back."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _weight(w: torch.Tensor | None, dim: int, device: int) -> int | None:
     if w is None:
         return None
@@ -134,13 +143,13 @@ class AttentionKernels:
         rows, q_heads, dim = q.shape
         dtype, at = q.dtype, self._here(rotary)
         if q_out is None:
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            q_out = _empty(q.shape, dtype, q.device, stream)
         _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
         if positions is not None:
             _need(positions.dtype is torch.int32 and positions.numel() == rows and positions.is_contiguous() and positions.get_device() == at, "positions: int32 [rows] on the kernels' device")
         if k is not None:
             if k_out is None:
-                k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+                k_out = _empty(k.shape, dtype, k.device, stream)
             k_heads = k.shape[1]
             _need(k_out.shape[1] == k_heads, "k_out has as many heads as k")
             k_args = (k.data_ptr(), k_out.data_ptr(), _row_stride(k, rows, dim, dtype, "k", at), _row_stride(k_out, rows, dim, dtype, "k_out", at), k_heads)
@@ -160,7 +169,7 @@ class AttentionKernels:
         _need(k.shape[1] == cache.kv_heads and v.shape[1] == cache.kv_heads, "k and v have the cache's heads")
         if q is not None:
             if q_out is None:
-                q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                q_out = _empty(q.shape, dtype, q.device, stream)
             q_heads = q.shape[1]
             _need(q_out.shape[1] == q_heads, "q_out has as many heads as q")
             q_args = (q.data_ptr(), q_out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(q_out, rows, dim, dtype, "q_out", at), q_heads,
@@ -178,9 +187,9 @@ class AttentionKernels:
         """The values of the cached tokens at the rows' positions; returns (k_out, v_out)."""
         rows, heads, dim, at = sequences.rows, cache.kv_heads, cache.head_dim, self._here(cache, sequences)
         if k_out is None:
-            k_out = torch.empty((rows, heads, dim), dtype=dtype, device=cache.pool.device)
+            k_out = _empty((rows, heads, dim), dtype, cache.pool.device, stream)
         if v_out is None:
-            v_out = torch.empty((rows, heads, dim), dtype=k_out.dtype, device=cache.pool.device)
+            v_out = _empty((rows, heads, dim), k_out.dtype, cache.pool.device, stream)
         dtype = k_out.dtype
         _need(k_out.shape[1] == heads and v_out.shape[1] == heads, "k_out and v_out have the cache's heads")
         status = self.lib.padra_kv_read(
@@ -190,28 +199,29 @@ class AttentionKernels:
             raise B.PadraError(status, "padra_kv_read")
         return k_out, v_out
 
-    def workspace(self, head_dim, stream):
-        """(address, bytes) of the workspace of calls on `stream` (a stream handle): calls on one stream follow one another.  It is
-        made by the first call on the stream, which therefore comes before any capture; captured calls keep using it, so
-        graphs captured on one stream are not to be replayed side by side."""
-        found = self._workspace.get((stream, head_dim))
+    def workspace(self, head_dim, handle, stream=None):
+        """(address, bytes) of the workspace of calls on `stream` (None: the current one), whose handle is given: calls on one
+        stream follow one another.  It is made by the first call on the stream, which therefore comes before any capture;
+        captured calls keep using it, so graphs captured on one stream are not to be replayed side by side."""
+        found = self._workspace.get((handle, head_dim))
         if found is None:
-            _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
+            with torch.cuda.stream(stream):
+                _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
             n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
-            ws = torch.empty(n, dtype=torch.uint8, device=self.bad.device)
-            found = self._workspace[stream, head_dim] = ws.data_ptr(), n, ws
+            ws = _empty((n,), torch.uint8, self.bad.device, stream)
+            found = self._workspace[handle, head_dim] = ws.data_ptr(), n, ws
         return found[:2]
 
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
         """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
         rows, dim, dtype, heads, at = sequences.rows, cache.head_dim, q.dtype, q.shape[1], self._here(cache, sequences)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = _empty(q.shape, dtype, q.device, stream)
         _need(out.shape[1] == heads, "out has as many heads as q")
-        stream = self._stream(stream)
+        handle = self._stream(stream)
         status = self.lib.padra_attention_q4(
             cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(out, rows, dim, dtype, "out", at), heads,
-            ROWS_TYPE.get(dtype, -1), scale, window, *self.workspace(dim, stream), self._bad, stream)
+            ROWS_TYPE.get(dtype, -1), scale, window, *self.workspace(dim, handle, stream), self._bad, handle)
         if status:
             raise B.PadraError(status, "padra_attention_q4")
         return out

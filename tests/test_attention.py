@@ -676,3 +676,22 @@ def test_values_on_and_beside_the_borders_of_codes(gpu):
         for h in range(2):
             R.store(want, int(c.table[0, r // 16]), h, r % 16, 16, c.k[r, h].double(), c.v[r, h].double())
     assert torch.equal(c.cache.pool.cpu(), want) and c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+def test_results_of_a_call_on_another_stream_are_that_streams_memory(gpu):
+    """Blocks that the current stream has just given back may still be in use there: the call's results do not take them."""
+    c = Call(gpu, [(1, 400), (30, 200)], 4, 2, 64, 16, torch.bfloat16, 97)
+    q, side = c.dq.contiguous(), torch.cuda.Stream()
+    want = c.kernels.attention(c.cache, c.sequences, q, 0.1)
+    k, v = c.kernels.read(c.cache, c.sequences)
+    rope = c.kernels.qk_norm_rope(q, k, None)
+    torch.cuda.synchronize()
+    held = [torch.empty_like(q) for _ in range(8)] + [torch.empty_like(k) for _ in range(8)]
+    freed = {t.data_ptr() for t in held}
+    del held
+    got = (c.kernels.attention(c.cache, c.sequences, q, 0.1, stream=side), *c.kernels.read(c.cache, c.sequences, stream=side),
+           *c.kernels.qk_norm_rope(q, k, None, stream=side), c.kernels.append(c.cache, c.sequences, c.dk, c.dv, q=q, stream=side))
+    side.synchronize()
+    assert not freed & {t.data_ptr() for t in got}
+    assert all(torch.equal(x, y) for x, y in zip(got, (want, k, v, *rope, q)))
