@@ -129,6 +129,9 @@ template <int D> struct Smem {
   alignas(1024) unsigned char k[kStages][kHalves][kTile * 128];
   alignas(1024) unsigned char v[kStages][kHalves][kTile * 128];
   alignas(8) unsigned long long q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages], s_full[2], p_full[2], o_full[2];
+  // A piece's queries may be replaced: its last S is done, and every softmax warp has seen them come and read its `column`.  Without the
+  // softmax warps' share a run of short pieces could stage queries twice while a warp still wrote rows out, and its wait, which knows
+  // one phase from the next only, would have taken the later staging for none.
   unsigned long long q_empty;
   unsigned long long shared_ready, shared_done; // the second half's maximum and sum are there / have been used
   struct {
@@ -447,7 +450,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
       BarrierInit(&sm.k_full[i], kProducerWarps), BarrierInit(&sm.v_full[i], kProducerWarps);
       BarrierInit(&sm.k_empty[i], 1), BarrierInit(&sm.v_empty[i], 1);
     }
-    BarrierInit(&sm.q_empty, 1);
+    BarrierInit(&sm.q_empty, 1 + kSoftmaxWarps);
     BarrierInit(&sm.shared_ready, kSoftmaxWarps / 2), BarrierInit(&sm.shared_done, kSoftmaxWarps / 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -499,7 +502,7 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           low = 0x7fffffff; // no token of the warp counts
       }
     };
-    // A piece's queries come before its first tile: this warp's 32 columns, once the MMAs of the piece before are done with Q.
+    // A piece's queries come before its first tile: this warp's 32 columns, once nobody needs those of the piece before.
     unsigned pieces = 0;
     auto stage_queries = [&]() {
       const int column0 = 32 * (warp - kSoftmaxWarps);
@@ -657,6 +660,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
         break;
       const float factor = sm.column[pieces & 1][own].factor;
       const int last = sm.column[pieces & 1][own].last, first = a.window ? max(0, last - a.window + 1) : 0;
+      __syncwarp();
+      if (lane == 0)
+        BarrierArrive(&sm.q_empty);
       float top = kNever, total = 0;
       const int least = __reduce_min_sync(0xffffffffu, there ? last : 0x7fffffff), latest = __reduce_max_sync(0xffffffffu, there ? first : 0);
       const int first_tile = walk.unit.first + walk.skip;

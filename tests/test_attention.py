@@ -695,3 +695,24 @@ def test_results_of_a_call_on_another_stream_are_that_streams_memory(gpu):
     side.synchronize()
     assert not freed & {t.data_ptr() for t in got}
     assert all(torch.equal(x, y) for x, y in zip(got, (want, k, v, *rope, q)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads, dim, page", [(8, 2, 64, 16), (8, 2, 128, 64), (3, 1, 64, 32)])
+@pytest.mark.parametrize("kind", ["one column block of 128", "blocks of more than 128", "both"])
+def test_runs_of_many_short_units_on_one_cta(gpu, heads, kv_heads, dim, page, kind):
+    """A prompt whose units are cut, then so many short ones that a CTA (one per SM) has four and more units of one to three tiles in its
+    run: blocks of at most 128 columns, in which both halves work on the same columns, larger ones, and both kinds in turn."""
+    g = torch.Generator().manual_seed(101 + dim)
+    group, shapes = heads // kv_heads, [(200, 1500)]
+    for i in range(800 // kv_heads):
+        wide = kind == "blocks of more than 128" or kind == "both" and bool(torch.rand(1, generator=g) < 0.5)
+        rows = int(torch.randint(128 // group + 1, 160 // group, (1,), generator=g)) if wide else int(torch.randint(1, 128 // group + 1, (1,), generator=g))
+        far = i % 7 == 3  # two or three tiles now and then
+        shapes.append((rows, rows + int(torch.randint(128 if far else 0, 260 if far else 128 - rows + 1, (1,), generator=g))))
+    c = Call(gpu, shapes, heads, kv_heads, dim, page, torch.bfloat16, 103, spare_rows=1)
+    first = c.check_attention()
+    for _ in range(30):
+        out = torch.full_like(first, 7.0)
+        assert torch.equal(c.kernels.attention(c.cache, c.sequences, c.dq, dim ** -0.5, out=out), first)
+    assert c.kernels.bad_flag() == 0
