@@ -136,8 +136,10 @@ __device__ __forceinline__ void TmemLoad4x8(unsigned taddr, float (&v)[4][8]) {
 #pragma unroll
   for (int q = 0; q < 4; ++q)
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < 8; ++j) {
+      asm volatile("" : "+r"(r[q][j])); // no use of a value moves up across the wait
       v[q][j] = __uint_as_float(r[q][j]);
+    }
 }
 
 

@@ -80,8 +80,10 @@ __device__ __forceinline__ void TmemLoad32(unsigned taddr, float (&v)[32]) {
                : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < 32; ++i) {
+    asm volatile("" : "+r"(r[i])); // no use of a value moves up across the wait
     v[i] = __uint_as_float(r[i]);
+  }
 }
 __device__ __forceinline__ void TmemStore32(unsigned taddr, const float (&v)[32]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
