@@ -8,6 +8,7 @@ qk_rope_* kernels (src/cuda/), which neither run on this GPU nor know pages or a
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -118,6 +119,7 @@ class AttentionKernels:
         self.bad = torch.zeros(1, dtype=torch.int32, device=device)
         self._bad, self._device = self.bad.data_ptr(), self.bad.get_device()
         self._workspace = {}  # (stream, head_dim) -> workspace: calls on one stream follow one another
+        self._making = threading.Lock()  # of a workspace: two threads' first calls on a stream have to get the same
 
     def reset_bad(self):
         self.bad.zero_()
@@ -202,15 +204,20 @@ class AttentionKernels:
     def workspace(self, head_dim, handle, stream=None):
         """(address, bytes) of the workspace of calls on `stream` (None: the current one), whose handle is given: calls on one
         stream follow one another.  It is made by the first call on the stream, which therefore comes before any capture;
-        captured calls keep using it, so graphs captured on one stream are not to be replayed side by side."""
+        captured calls keep using it, so graphs captured on one stream are not to be replayed side by side, nor beside calls on it."""
         found = self._workspace.get((handle, head_dim))
         if found is None:
-            with torch.cuda.stream(stream):
-                _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
-            n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
-            ws = _empty((n,), torch.uint8, self.bad.device, stream)
-            found = self._workspace[handle, head_dim] = ws.data_ptr(), n, ws
+            with self._making:
+                found = self._workspace.get((handle, head_dim)) or self._make_workspace(head_dim, handle, stream)
         return found[:2]
+
+    def _make_workspace(self, head_dim, handle, stream):
+        with torch.cuda.stream(stream):
+            _need(not torch.cuda.is_current_stream_capturing(), "the first attention call on a stream allocates its workspace: make it before capturing")
+        n = self.lib.padra_attention_q4_workspace_bytes(head_dim)
+        ws = _empty((n,), torch.uint8, self.bad.device, stream)
+        self._workspace[handle, head_dim] = made = ws.data_ptr(), n, ws
+        return made
 
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
         """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""

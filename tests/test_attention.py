@@ -2,6 +2,8 @@
 (tests/attention_reference.py).  The refusals run on the CPU: they come from the C ABI's argument checks."""
 import ctypes as C
 import math
+import threading
+import time
 
 import pytest
 import torch
@@ -113,6 +115,27 @@ def test_python_side_checks_shapes_and_types():
         A.Sequences(i[None], i, i, 4, 4)
     with pytest.raises(ValueError):
         A.Sequences(torch.zeros((3, 1), dtype=torch.int64), torch.zeros(4, dtype=torch.int32), i, 4, 4)
+
+
+def test_first_calls_of_two_threads_get_one_workspace(monkeypatch):
+    from types import SimpleNamespace
+
+    from padra_b200 import attention as A
+
+    def slowly(head_dim):
+        time.sleep(0.05)
+        return 4096
+
+    k = A.AttentionKernels.__new__(A.AttentionKernels)  # without a device
+    k.lib, k.bad, k._workspace, k._making = SimpleNamespace(padra_attention_q4_workspace_bytes=slowly), torch.zeros(1), {}, threading.Lock()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(k.workspace(64, 0))) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 4 and set(got) == {(k._workspace[0, 64][0], 4096)}
 
 
 def test_reference_quantiser_against_a_plain_loop():
