@@ -392,7 +392,8 @@ PADRA_API int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *
  * head g); out may not overlap q.  Call after the rows' own K and V have been appended.  A query that is not finite raises
  * *bad and gives zeros.
  * workspace: padra_attention_q4_workspace_bytes(head_dim) bytes (the same for every call), 16-byte aligned; what it holds before
- * a call does not matter.  Calls that share it, captured ones among them, must not overlap on the GPU. */
+ * a call does not matter.  Calls that share it, captured ones among them, must not overlap on the GPU; several host threads
+ * may issue theirs on one stream. */
 PADRA_API size_t padra_attention_q4_workspace_bytes(int head_dim);
 PADRA_API int padra_attention_q4(const padra_kv_cache *cache, const padra_sequences *sequences, const void *q, void *out,
                                  long long q_stride, long long out_stride, int q_heads, int type, float scale,

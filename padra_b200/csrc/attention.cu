@@ -23,6 +23,7 @@
 // Measured: 64 sequences of 1 to 16384 tokens, 32 heads over 4, head size 128: 81 us, 3.8 TB/s of codes and scales (58% of a copy), bound by
 // instruction issue; one sequence of 131072 tokens: 24 us and 7 us for the join; of 4097: 13 us, all latency.
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #include "attention.cuh"
@@ -551,6 +552,13 @@ constexpr size_t kSplitBytes = kMaxGrid * sizeof(Split);
 static_assert(kSplitBytes % 16 == 0, "the pieces behind are read 16 bytes at a time");
 constexpr int kMaxColumns = 16;
 
+// A call is two launches, and the second reads what the first has left in the workspace.  Host threads that share a workspace on one
+// stream take turns here: a call's first launch may not come between the two of another.
+std::mutex &OrderOf(const void *workspace) {
+  static std::mutex order[64];
+  return order[reinterpret_cast<uintptr_t>(workspace) / 256 % 64];
+}
+
 } // namespace
 
 size_t AttentionWorkspaceBytes(int head_dim) {
@@ -581,6 +589,7 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
   AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * 1.4426950408889634f : 1.f,
                   scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f, window,
                   static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), kCodeMasks, bad};
+  const std::lock_guard<std::mutex> turn(OrderOf(workspace));
   if (type == PADRA_ROWS_BF16)
     return c.head_dim == 64 ? LaunchColumns<__nv_bfloat16, 64>(a, sms, stream) : LaunchColumns<__nv_bfloat16, 128>(a, sms, stream);
   return c.head_dim == 64 ? LaunchColumns<__half, 64>(a, sms, stream) : LaunchColumns<__half, 128>(a, sms, stream);

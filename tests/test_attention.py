@@ -739,3 +739,27 @@ def test_runs_of_many_short_units_on_one_cta(gpu, heads, kv_heads, dim, page, ki
         out = torch.full_like(first, 7.0)
         assert torch.equal(c.kernels.attention(c.cache, c.sequences, c.dq, dim ** -0.5, out=out), first)
     assert c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+def test_two_threads_on_one_stream(gpu):
+    """Calls with many cut units, whose joins read the workspace that the threads share: each gets its own results."""
+    calls = [Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 107 + i) for i, shapes in enumerate(([(1, 3000)] * 3, [(1, 5000), (2, 900)], [(100, 700), (30, 2000)]))]
+    kernels = calls[0].kernels
+    alone = [kernels.attention(c.cache, c.sequences, c.dq, 0.1) for c in calls]
+    torch.cuda.synchronize()
+    outs, start = [[] for _ in calls], threading.Barrier(len(calls))
+
+    def work(c, out):
+        start.wait()
+        for _ in range(400):
+            out.append(kernels.attention(c.cache, c.sequences, c.dq, 0.1))
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(calls, outs)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(kernels._workspace) == 1 and kernels.bad_flag() == 0
+    for out, want in zip(outs, alone):
+        assert len(out) == 400 and all(torch.equal(x, want) for x in out)
