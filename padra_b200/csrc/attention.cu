@@ -201,7 +201,7 @@ template <typename T, int D, int NT> struct Piece {
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sums[i] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
       }
-      const float mine = a.scale * ldexpf(1.f, exponent);
+      const float mine = FactorOf(a.scale, ldexpf(1.f, exponent));
       // a row at a negative position sees nothing, nor does one that is not finite, nor a column beyond the last
       const int to = column < columns && fine ? start + row : -1, from = a.window ? max(0, to - a.window + 1) : 0;
 #pragma unroll

@@ -10,6 +10,7 @@ namespace attention {
 
 constexpr float kNever = -1e30f; // the running maximum before any token
 constexpr float kTop = 8.f, kRaise = 15.f; // log2 of the largest weight after a raise / before the next
+constexpr float kLeastFactor = 0x1p-126f;  // of scores: see FactorOf
 constexpr int kMaxGrid = 512, kMaxWideGrid = 160; // CTAs that the workspace provides for, of either kernel
 
 // Two codes as FP16 numbers: nibbles 0 and 4 of a word become 1024 + n, nibbles 1 and 5 become 64 + n, one logic operation each.
@@ -60,6 +61,11 @@ __device__ __forceinline__ float Exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// What a column's scores are multiplied by.  It does not become zero, which would make a NaN of a masked token's -infinity; at the least
+// factor every score (below 2^25 before the factor) is as good as zero.
+__device__ __forceinline__ float FactorOf(float scale, float power) {
+  return fmaxf(scale * power, kLeastFactor);
 }
 __device__ __forceinline__ void Widen(uint4 u, const __nv_bfloat16 *, float (&x)[8]) {
   const unsigned w[4] = {u.x, u.y, u.z, u.w};

@@ -388,7 +388,7 @@ __device__ __forceinline__ void StageQueries(const AttentionArgs &a, const Rows 
       if (piece == 0) {
         if (!finite)
           Raise(a.bad);
-        sm.column[parity][c].factor = a.scale * (finite ? power : 1.f);
+        sm.column[parity][c].factor = FactorOf(a.scale, finite ? power : 1.f);
         sm.column[parity][c].last = c < columns && finite ? position[f] : -1;
       }
     }

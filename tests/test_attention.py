@@ -763,3 +763,14 @@ def test_two_threads_on_one_stream(gpu):
     assert len(kernels._workspace) == 1 and kernels.bad_flag() == 0
     for out, want in zip(outs, alone):
         assert len(out) == 400 and all(torch.equal(x, want) for x in out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(1, 300), (3, 40)], [(40, 300), (130, 140)]])  # few and many columns
+@pytest.mark.parametrize("value, scale", [(0.0, 1e-8), (1e-38, 1e-3), (1e-38, 1e-20), (-1.0, 1e-38), (1e-30, -1e-30)])
+def test_scores_too_small_for_32_bits_give_equal_weights(gpu, shapes, value, scale):
+    c = Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 109)
+    c.q[:] = value
+    c.d_qkv.copy_(c.qkv)
+    c.check_attention(scale=scale)
+    c.check_attention(scale=scale, window=30)
