@@ -318,6 +318,8 @@ template <typename T, int D, int NT> struct Piece {
             for (int m = 4; m < 32; m *= 2)
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
             const float next = fmaxf(top[n][e], fmaf(x, factor[n][e], -kTop)), shrink = Exp2(top[n][e] - next);
+            if (next > kNever && fabsf(next) > kLargestTop)
+              Raise(a.bad);
             top[n][e] = next, sum[n][e] *= shrink;
 #pragma unroll
             for (int t = 0; t < 2 * kChunks; ++t)
@@ -551,6 +553,7 @@ template <typename T, int D> int LaunchColumns(const AttentionArgs &a, int sms, 
 constexpr size_t kSplitBytes = kMaxGrid * sizeof(Split);
 static_assert(kSplitBytes % 16 == 0, "the pieces behind are read 16 bytes at a time");
 constexpr int kMaxColumns = 16;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // A call is two launches, and the second reads what the first has left in the workspace.  Host threads that share a workspace on one
 // stream take turns here: a call's first launch may not come between the two of another.
@@ -573,7 +576,7 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
   KvView c;
   SequenceView s;
   if (!ViewOf(cache, &c) || !ViewOf(sequences, c, &s) || !bad || q_heads < 1 || q_heads > 4096 || q_heads % c.kv_heads || window < 0 ||
-      !std::isfinite(scale))
+      !std::isfinite(scale * kLog2e))
     return PADRA_INVALID_ARGUMENT;
   if ((c.head_dim != 64 && c.head_dim != 128) || (type != PADRA_ROWS_BF16 && type != PADRA_ROWS_F16))
     return PADRA_UNSUPPORTED;
@@ -586,7 +589,7 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
   int device = 0, sms = 0;
   if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
     return PADRA_INTERNAL;
-  AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * 1.4426950408889634f : 1.f,
+  AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * kLog2e : 1.f,
                   scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f, window,
                   static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), kCodeMasks, bad};
   const std::lock_guard<std::mutex> turn(OrderOf(workspace));

@@ -10,7 +10,9 @@ namespace attention {
 
 constexpr float kNever = -1e30f; // the running maximum before any token
 constexpr float kTop = 8.f, kRaise = 15.f; // log2 of the largest weight after a raise / before the next
-constexpr float kLeastFactor = 0x1p-126f;  // of scores: see FactorOf
+constexpr float kLeastFactor = 0x1p-126f, kLargestFactor = 0x1p64f; // of scores: see FactorOf
+constexpr float kLargestTop = 0x1p24f; // the largest magnitude of a running maximum, in log2: beyond it weights next to each other are
+                                       // more than a factor of two apart, and soon none is finite
 constexpr int kMaxGrid = 512, kMaxWideGrid = 160; // CTAs that the workspace provides for, of either kernel
 
 // Two codes as FP16 numbers: nibbles 0 and 4 of a word become 1024 + n, nibbles 1 and 5 become 64 + n, one logic operation each.
@@ -63,9 +65,10 @@ __device__ __forceinline__ float Exp2(float x) {
   return y;
 }
 // What a column's scores are multiplied by.  It does not become zero, which would make a NaN of a masked token's -infinity; at the least
-// factor every score (below 2^25 before the factor) is as good as zero.
+// factor every score (below 2^25 before the factor) is as good as zero.  At the largest they stay above kNever; a score that is not zero is
+// beyond kLargestTop there, or lost in 32 bits.
 __device__ __forceinline__ float FactorOf(float scale, float power) {
-  return fmaxf(scale * power, kLeastFactor);
+  return fminf(fmaxf(scale * power, kLeastFactor), kLargestFactor);
 }
 __device__ __forceinline__ void Widen(uint4 u, const __nv_bfloat16 *, float (&x)[8]) {
   const unsigned w[4] = {u.x, u.y, u.z, u.w};

@@ -702,6 +702,8 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
           const bool raise = fmaf(most, factor, -top) > kRaise;
           if (__any_sync(0xffffffffu, raise)) {
             const float next = raise ? fmaf(most, factor, -kTop) : top, shrink = Exp2(top - next);
+            if (raise && fabsf(next) > kLargestTop)
+              Raise(a.bad);
             top = next;
 #pragma unroll
             for (int k = 0; k < 2; ++k)

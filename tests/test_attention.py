@@ -774,3 +774,60 @@ def test_scores_too_small_for_32_bits_give_equal_weights(gpu, shapes, value, sca
     c.d_qkv.copy_(c.qkv)
     c.check_attention(scale=scale)
     c.check_attention(scale=scale, window=30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(1, 300), (3, 40)], [(40, 300), (130, 140)]])
+@pytest.mark.parametrize("value, scale", [(3e38, 0.1), (1e10, 1e30), (-1e20, 1e20), (1e9, 1.0)])
+def test_scores_too_large_for_32_bits_are_reported(gpu, shapes, value, scale):
+    c = Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 113)
+    c.q[:] = value
+    c.d_qkv.copy_(c.qkv)
+    for sign in (1, -1):
+        c.kernels.attention(c.cache, c.sequences, c.dq, sign * scale)
+        assert c.kernels.bad_flag() == 1
+        c.kernels.reset_bad()
+    a, b = 64 * 64, 64 * 8  # keys of zero: all scores are
+    c.pool[:, :, a:a + b] = 0
+    c.cache.pool.copy_(c.pool)
+    c.check_attention(scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(1, 300), (3, 40)], [(40, 300), (130, 140)]])
+@pytest.mark.parametrize("level", [-1.0, 1.0])
+def test_large_scores_that_differ_by_little(gpu, shapes, level):
+    """Scores of +-3.5 * 2^20 and 0 to 4 more, in the exponent of two.  Every product and sum is exact in 32 bits, so the weights are 2^(t % 5)
+    up to their rounding to FP16 (2^-11, as V's) whatever the size of the scores."""
+    c = Call(gpu, shapes, 8, 2, 128, 64, torch.bfloat16, 127)
+    c.q[:] = 0
+    c.q[:, :, 0], c.q[:, :, 32] = 2.0 ** 20 * level, 1.0
+    c.d_qkv.copy_(c.qkv)
+    for s, (_, ctx) in enumerate(shapes):
+        for t in range(ctx):
+            k = torch.zeros(128, dtype=torch.float64)
+            k[0], k[32], k[33] = 3.5, t % 5, 7.0  # steps of 0.5 and 1
+            page, slot = int(c.table[s, t // 64]), t % 64
+            values = R.fetch(c.pool, page, 64, 128)[1]
+            for h in range(2):
+                R.store(c.pool, page, h, slot, 64, k, values[h, slot])
+    c.cache.pool.copy_(c.pool)
+    out = c.kernels.attention(c.cache, c.sequences, c.dq, math.log(2)).cpu().double()
+    assert c.kernels.bad_flag() == 0
+    for s, (n, ctx) in enumerate(shapes):
+        v = R.tokens(c.pool, c.table[s], ctx, 64, 128)[1].repeat_interleave(4, 1)
+        for r in range(n):
+            seen = v[:ctx - n + r + 1]
+            p = 2.0 ** (torch.arange(len(seen)) % 5).double()
+            p = (p / p.sum())[:, None, None]
+            want, bound = (p * seen).sum(0), 2 * 3 * 2 ** -11 * (p * seen.abs()).sum(0)
+            assert ((out[int(c.begin[s]) + r] - want).abs() <= bound + 2.0 ** -8 * want.abs()).all()
+
+
+def test_a_scale_that_leaves_32_bits_is_refused(lib):
+    from padra_b200 import binding as B
+
+    c, s, _ = structs(rows=0)
+    p = 4096
+    for scale, want in ((3e38, B.INVALID_ARGUMENT), (-3e38, B.INVALID_ARGUMENT), (2e38, B.OK)):
+        assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, scale, 0, p, 1 << 40, p, None) == want
