@@ -144,17 +144,43 @@ struct Weights {
     Rows<__nv_bfloat16>::Unpack(__ldg(reinterpret_cast<const uint2 *>(weight + lane.hi)), w + 4);
   }
 };
+// Sum over the D / 8 lanes of a head.
+template <int D> __device__ __forceinline__ float HeadSum(float x) {
+#pragma unroll
+  for (int d = 1; d < D / 8; d *= 2)
+    x += __shfl_xor_sync(0xffffffffu, x, d);
+  return x;
+}
 template <int D, bool Interleaved>
-__device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool normed, const Weights &weights, float eps, const Turn<float> (&turns)[4]) {
+__device__ __forceinline__ void NormRotate(float (&x)[8], const Lane &lane, bool normed, const Weights &weights, double eps, const Turn<float> (&turns)[4]) {
   if (normed) {
     float sum = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       sum += x[i] * x[i];
+    const float mean = HeadSum<D>(sum) * (1.f / D) + static_cast<float>(eps);
+    float inverse = rsqrtf(mean);
+    // Squares of values beyond 2^64 are infinite in 32 bits, those of small ones lose bits or vanish beside a small eps.  Such a head is
+    // multiplied by a power of two first; the whole warp goes there, with a factor of one for its other heads.
+    const bool narrow = mean >= 0x1p-100f && mean <= 0x1p100f;
+    if (__any_sync(0xffffffffu, !narrow)) {
+      float most = sqrtf(static_cast<float>(eps));
 #pragma unroll
-    for (int d = 1; d < D / 8; d *= 2)
-      sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    const float inverse = rsqrtf(sum * (1.f / D) + eps);
+      for (int i = 0; i < 8; ++i)
+        most = fmaxf(most, fabsf(x[i]));
+#pragma unroll
+      for (int d = 1; d < D / 8; d *= 2)
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      // 2^-k for most in [2^k, 2^(k + 1)), within 2^-126 .. 2^126: the exponent's bits from those of 2^254
+      const float power = narrow ? 1.f : __uint_as_float((254u << 23) - min(max(__float_as_uint(most) & 0x7f800000u, 1u << 23), 253u << 23));
+      sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] *= power, sum += x[i] * x[i];
+      sum = HeadSum<D>(sum);
+      if (!narrow)
+        inverse = rsqrtf(sum * (1.f / D) + static_cast<float>(eps * power * power));
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       x[i] = x[i] * inverse * weights.w[i];
@@ -196,7 +222,7 @@ template <typename T, int D, int Ahead> struct UnitLoop {
     in += stride * D;
   }
   template <bool Interleaved, typename Turns>
-  __device__ __forceinline__ void Run(const HeadRows &a, long long row, const Lane &lane, float eps, const Turns &turns_of_row, int *bad) {
+  __device__ __forceinline__ void Run(const HeadRows &a, long long row, const Lane &lane, double eps, const Turns &turns_of_row, int *bad) {
     Weights weights{};
     Turn<float> turns[4] = {};
     const bool normed = a.weight != nullptr;
@@ -244,8 +270,9 @@ __device__ __forceinline__ int After(int first, int units, int step) { // the fi
   return first >= units ? first - units : (first - units) % step + (((first - units) % step) ? step : 0);
 }
 
+// Three CTAs an SM at 80 registers with 20 bytes spilled; left to itself the compiler takes 89, for two (16384 rows: a call of 74 us instead of 68).
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) NormRopeKernel(HeadRows q, HeadRows k, float eps, const int *positions, RotaryArgs rotary, int rows,
+__global__ void __launch_bounds__(kRowThreads, sizeof(T) == 2 ? 3 : 2) NormRopeKernel(HeadRows q, HeadRows k, double eps, const int *positions, RotaryArgs rotary, int rows,
                                                               int row_warps, int *bad) {
   constexpr int kSide = 32 / (D / 8);
   __shared__ __align__(16) Turn<float> turns[kMaxCtaRows][D / 2];
@@ -423,9 +450,9 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
   if (share.row >= count || s_page[share.row] < 0)
     return;
   if (rotary.interleaved)
-    q_loop.template Run<true>(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
+    q_loop.template Run<true>(q, row, q_lane, eps, q_turns[share.row], bad);
   else
-    q_loop.template Run<false>(q, row, q_lane, static_cast<float>(eps), q_turns[share.row], bad);
+    q_loop.template Run<false>(q, row, q_lane, eps, q_turns[share.row], bad);
   const int slot = s_position[share.row] & (cache.page_size - 1), group = at / 4, quarter = at & 3;
   for (; unit < 2 * kv_units; unit += share.step) { // warp-uniform up to the head
     const bool is_v = unit >= kv_units;
@@ -561,7 +588,7 @@ template <typename T, int D> struct NormRope {
     int row_warps;
     dim3 grid;
     Shape(rows, (q.heads + kSide - 1) / kSide + (k.heads + kSide - 1) / kSide, &row_warps, &grid);
-    NormRopeKernel<T, D><<<grid, kRowThreads, 0, stream>>>(q, k, static_cast<float>(eps), positions, rotary, rows, row_warps, bad);
+    NormRopeKernel<T, D><<<grid, kRowThreads, 0, stream>>>(q, k, eps, positions, rotary, rows, row_warps, bad);
     return CudaStatus(cudaGetLastError());
   }
 };

@@ -831,3 +831,41 @@ def test_a_scale_that_leaves_32_bits_is_refused(lib):
     p = 4096
     for scale, want in ((3e38, B.INVALID_ARGUMENT), (-3e38, B.INVALID_ARGUMENT), (2e38, B.OK)):
         assert lib.padra_attention_q4(C.byref(c), C.byref(s), p, p, 512, 512, 4, 0, scale, 0, p, 1 << 40, p, None) == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim, interleaved", [(64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("eps", [1e-6, 1e-30, 0.0])
+def test_norm_of_values_whose_squares_leave_32_bits(gpu, dtype, dim, interleaved, eps):
+    """Heads of ordinary size among others up to 1e38 and down to 1e-38: each as its formula gives it, whatever its neighbours are."""
+    from padra_b200 import attention as A
+
+    g = torch.Generator().manual_seed(131 + dim)
+    rows, heads = 9, 7
+    x = torch.randn((rows, heads, dim), generator=g).double()
+    size = torch.tensor([1.0, 1e18, 1e20, 1e36, 1e-19, 1e-25, 1e-36], dtype=torch.float64)
+    plain = x.to(dtype)
+    x = (x * size[torch.stack([torch.randperm(7, generator=g) for _ in range(rows)])][..., None]).to(dtype)
+    weight = (1 + 0.3 * torch.randn(dim, generator=g)).bfloat16()
+    inv_freq, amplitude = R.yarn_like(dim // 2, 2.0)
+    positions = torch.arange(rows, dtype=torch.int32)
+    kernels, rotary = A.AttentionKernels(gpu), A.Rotary(inv_freq.to(gpu), interleaved, amplitude)
+    got = kernels.qk_norm_rope(x.to(gpu), x.to(gpu), positions.to(gpu), rotary, weight.to(gpu), weight.to(gpu), eps)
+    normed = R.rms(x, weight, eps)
+    want = R.rotate(normed, positions, inv_freq, interleaved, amplitude)
+    # as in test_norm_and_rotation; a BF16 value below the normal range is off by half a step of 2^-133
+    slack = 2.0 ** -19 * 2 * amplitude * normed.abs().amax(-1, keepdim=True) + 2.0 ** -134
+    for y in got:
+        assert ((y.cpu().double() - want).abs() <= HALF[dtype] * want.abs() + slack).all()
+    assert kernels.bad_flag() == 0
+    # an ordinary head's bits do not depend on what lies beside it
+    alone = kernels.qk_norm_rope(plain.to(gpu), None, positions.to(gpu), rotary, weight.to(gpu), None, eps)[0]
+    same = (x == plain).all(-1)
+    assert same.any() and torch.equal(got[0].cpu()[same], alone.cpu()[same])
+    if dim < 256:  # the queries of an append
+        begin, context = torch.tensor([0, rows], dtype=torch.int32, device=gpu), torch.tensor([rows], dtype=torch.int32, device=gpu)
+        cache = A.KvCache(1, 16, 1, dim, gpu)
+        k = torch.ones((rows, 1, dim), dtype=dtype, device=gpu)
+        q = kernels.append(cache, A.Sequences(torch.zeros((1, 1), dtype=torch.int32, device=gpu), begin, context, rows, rows), k, k, rotary, weight.to(gpu), eps, x.to(gpu), weight.to(gpu))
+        assert ((q.cpu().double() - want).abs() <= HALF[dtype] * want.abs() + slack * math.sqrt(2)).all() and kernels.bad_flag() == 0
