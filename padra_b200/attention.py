@@ -15,6 +15,7 @@ import torch
 from . import binding as B
 
 GROUP = 32  # values that share an FP16 scale
+NO_WINDOW = 2 ** 31 - 1  # as wide as an int goes, wider than any context
 ROWS_TYPE = {torch.bfloat16: B.ROWS_BF16, torch.float16: B.ROWS_F16, torch.float32: B.ROWS_F32}
 
 
@@ -228,7 +229,7 @@ class AttentionKernels:
         handle = self._stream(stream)
         status = self.lib.padra_attention_q4(
             cache.ref, sequences.ref, q.data_ptr(), out.data_ptr(), _row_stride(q, rows, dim, dtype, "q", at), _row_stride(out, rows, dim, dtype, "out", at), heads,
-            ROWS_TYPE.get(dtype, -1), scale, window, *self.workspace(dim, handle, stream), self._bad, handle)
+            ROWS_TYPE.get(dtype, -1), scale, min(window, NO_WINDOW), *self.workspace(dim, handle, stream), self._bad, handle)
         if status:
             raise B.PadraError(status, "padra_attention_q4")
         return out

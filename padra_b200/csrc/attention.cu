@@ -590,7 +590,8 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
   if (cudaGetDevice(&device) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || sms < 1)
     return PADRA_INTERNAL;
   AttentionArgs a{c, s, q, out, q_stride, out_stride, q_heads, q_heads / c.kv_heads, scale ? fabsf(scale) * kLog2e : 1.f,
-                  scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f, window,
+                  scale > 0 ? 1.f : scale < 0 ? -1.f : 0.f,
+                  window >> 30 ? 0 : window, // positions are below 2^30: nothing is outside, and position - window stays in 32 bits
                   static_cast<Split *>(workspace), reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + kSplitBytes), kCodeMasks, bad};
   const std::lock_guard<std::mutex> turn(OrderOf(workspace));
   if (type == PADRA_ROWS_BF16)

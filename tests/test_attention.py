@@ -869,3 +869,11 @@ def test_norm_of_values_whose_squares_leave_32_bits(gpu, dtype, dim, interleaved
         k = torch.ones((rows, 1, dim), dtype=dtype, device=gpu)
         q = kernels.append(cache, A.Sequences(torch.zeros((1, 1), dtype=torch.int32, device=gpu), begin, context, rows, rows), k, k, rotary, weight.to(gpu), eps, x.to(gpu), weight.to(gpu))
         assert ((q.cpu().double() - want).abs() <= HALF[dtype] * want.abs() + slack * math.sqrt(2)).all() and kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(5, 2), (1, 40), (7, 3)], [(60, 10), (40, 300), (5, 0)]])  # more rows than context: few and many columns
+@pytest.mark.parametrize("window", [2 ** 40 + 1, 2 ** 31 - 1, 2 ** 31 - 8, 2 ** 30])
+def test_a_window_wider_than_any_context_is_none(gpu, shapes, window):
+    c = Call(gpu, shapes, 8, 2, 64, 16, torch.bfloat16, 137)
+    assert torch.equal(c.check_attention(window=window), c.check_attention())
