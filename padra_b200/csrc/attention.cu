@@ -580,7 +580,7 @@ int LaunchAttention(const padra_kv_cache *cache, const padra_sequences *sequence
     return PADRA_INVALID_ARGUMENT;
   if ((c.head_dim != 64 && c.head_dim != 128) || (type != PADRA_ROWS_BF16 && type != PADRA_ROWS_F16))
     return PADRA_UNSUPPORTED;
-  if (!RowsOk(q, q_stride, q_heads, c.head_dim) || !RowsOk(out, out_stride, q_heads, c.head_dim))
+  if (!RowsOk(q, q_stride, s.rows, q_heads, c.head_dim) || !RowsOk(out, out_stride, s.rows, q_heads, c.head_dim))
     return PADRA_INVALID_ARGUMENT;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < AttentionWorkspaceBytes(c.head_dim))
     return PADRA_INVALID_ARGUMENT;

@@ -635,12 +635,12 @@ int LaunchNormRope(const void *q, void *q_out, long long q_stride, long long q_o
                    cudaStream_t stream) {
   RotaryArgs r;
   if (rows < 0 || rows > (1 << 24) || q_heads < 1 || q_heads > 4096 || k_heads < 0 || k_heads > 4096 || !bad || !(eps >= 0) ||
-      !RotaryOk(rotary, head_dim, &r) || (r.dims && !positions) || !WeightOk(q_weight) || !WeightOk(k_weight))
+      !RotaryOk(rotary, head_dim, &r) || (r.dims && rows && !positions) || !WeightOk(q_weight) || !WeightOk(k_weight))
     return PADRA_INVALID_ARGUMENT;
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return PADRA_UNSUPPORTED;
-  if (!RowsOk(q, q_stride, q_heads, head_dim) || !RowsOk(q_out, q_out_stride, q_heads, head_dim) ||
-      (k_heads && (!RowsOk(k, k_stride, k_heads, head_dim) || !RowsOk(k_out, k_out_stride, k_heads, head_dim))))
+  if (!RowsOk(q, q_stride, rows, q_heads, head_dim) || !RowsOk(q_out, q_out_stride, rows, q_heads, head_dim) ||
+      (k_heads && (!RowsOk(k, k_stride, rows, k_heads, head_dim) || !RowsOk(k_out, k_out_stride, rows, k_heads, head_dim))))
     return PADRA_INVALID_ARGUMENT;
   if (!rows)
     return PADRA_OK;
@@ -660,9 +660,9 @@ int LaunchKvAppend(const padra_kv_cache *cache, const padra_sequences *sequences
     return PADRA_INVALID_ARGUMENT;
   if (c.head_dim != 64 && c.head_dim != 128)
     return PADRA_UNSUPPORTED;
-  if (!RowsOk(k, k_stride, c.kv_heads, c.head_dim) || !RowsOk(v, v_stride, c.kv_heads, c.head_dim))
+  if (!RowsOk(k, k_stride, s.rows, c.kv_heads, c.head_dim) || !RowsOk(v, v_stride, s.rows, c.kv_heads, c.head_dim))
     return PADRA_INVALID_ARGUMENT;
-  if (q && (q_heads < 1 || q_heads > 4096 || !RowsOk(q, q_stride, q_heads, c.head_dim) || !RowsOk(q_out, q_out_stride, q_heads, c.head_dim)))
+  if (q && (q_heads < 1 || q_heads > 4096 || !RowsOk(q, q_stride, s.rows, q_heads, c.head_dim) || !RowsOk(q_out, q_out_stride, s.rows, q_heads, c.head_dim)))
     return PADRA_INVALID_ARGUMENT;
   if (!s.rows || !s.count)
     return PADRA_OK;
@@ -679,7 +679,7 @@ int LaunchKvRead(const padra_kv_cache *cache, const padra_sequences *sequences, 
     return PADRA_INVALID_ARGUMENT;
   if (c.head_dim != 64 && c.head_dim != 128)
     return PADRA_UNSUPPORTED;
-  if (!RowsOk(k_out, k_stride, c.kv_heads, c.head_dim) || !RowsOk(v_out, v_stride, c.kv_heads, c.head_dim))
+  if (!RowsOk(k_out, k_stride, s.rows, c.kv_heads, c.head_dim) || !RowsOk(v_out, v_stride, s.rows, c.kv_heads, c.head_dim))
     return PADRA_INVALID_ARGUMENT;
   if (!s.rows || !s.count)
     return PADRA_OK;

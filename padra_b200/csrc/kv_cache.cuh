@@ -46,8 +46,8 @@ inline bool ViewOf(const padra_sequences *s, const KvView &cache, SequenceView *
   *v = SequenceView{s->page_table, s->row_begin, s->context, s->count, s->table_stride, s->rows, s->max_rows};
   return true;
 }
-inline bool RowsOk(const void *p, long long stride, int heads, int head_dim) {
-  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && stride >= static_cast<long long>(heads) * head_dim;
+inline bool RowsOk(const void *p, long long stride, int rows, int heads, int head_dim) { // no rows need no memory
+  return (p || !rows) && reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride % 8 == 0 && stride >= static_cast<long long>(heads) * head_dim;
 }
 
 // Rows and context of sequence s, checked: false (and *bad raised) where they contradict the call.

@@ -101,6 +101,23 @@ def test_nothing_to_do_is_not_an_error(lib):
     assert lib.padra_qk_norm_rope(p, p, 256, 256, 4, None, None, 0, 0, 0, None, None, 1e-6, p, None, 0, 64, 0, p, None) == B.OK
 
 
+def test_row_arrays_without_rows_need_no_memory(lib):
+    """As a framework's empty tensors, whose address is null."""
+    from padra_b200 import binding as B
+
+    p = 4096
+    c, s, r = structs(rows=0)
+    assert lib.padra_attention_q4(C.byref(c), C.byref(s), None, None, 512, 512, 4, 0, 0.1, 0, p, 1 << 40, p, None) == B.OK
+    assert lib.padra_kv_read(C.byref(c), C.byref(s), None, None, 128, 128, 0, p, None) == B.OK
+    assert lib.padra_kv_append(C.byref(c), C.byref(s), None, None, 128, 128, None, 1e-6, C.byref(r), None, None, 256, 256, 4, None, 0, p, None) == B.OK
+    assert lib.padra_qk_norm_rope(None, None, 256, 256, 4, None, None, 128, 128, 2, None, None, 1e-6, None, C.byref(r), 0, 64, 0, p, None) == B.OK
+    # what is wrong in itself is refused all the same
+    assert lib.padra_attention_q4(C.byref(c), C.byref(s), None, None, 255, 512, 4, 0, 0.1, 0, p, 1 << 40, p, None) == B.INVALID_ARGUMENT
+    assert lib.padra_attention_q4(C.byref(c), C.byref(s), None, None, 512, 512, 4, B.ROWS_F32, 0.1, 0, p, 1 << 40, p, None) == B.UNSUPPORTED
+    assert lib.padra_kv_read(C.byref(c), C.byref(s), None, None, 120, 128, 0, p, None) == B.INVALID_ARGUMENT
+    assert lib.padra_qk_norm_rope(p + 4, None, 256, 256, 4, None, None, 0, 0, 0, None, None, 1e-6, None, None, 0, 64, 0, p, None) == B.INVALID_ARGUMENT
+
+
 def test_python_side_checks_shapes_and_types():
     from padra_b200 import attention as A
 
@@ -877,3 +894,21 @@ def test_norm_of_values_whose_squares_leave_32_bits(gpu, dtype, dim, interleaved
 def test_a_window_wider_than_any_context_is_none(gpu, shapes, window):
     c = Call(gpu, shapes, 8, 2, 64, 16, torch.bfloat16, 137)
     assert torch.equal(c.check_attention(window=window), c.check_attention())
+
+
+@pytest.mark.gpu
+def test_calls_without_rows(gpu):
+    c = Call(gpu, [(0, 30), (0, 0)], 8, 2, 64, 16, torch.bfloat16, 139, strided=False)
+    k, before = c.kernels, c.cache.pool.clone()
+    from padra_b200 import attention as A
+
+    rotary = A.Rotary(torch.ones(32, dtype=torch.float64, device=gpu))
+    empty = lambda heads: torch.empty((0, heads, 64), dtype=torch.bfloat16, device=gpu)  # noqa: E731
+    assert k.attention(c.cache, c.sequences, empty(8), 0.1).shape == (0, 8, 64)
+    assert k.append(c.cache, c.sequences, empty(2), empty(2), rotary, q=empty(8)).shape == (0, 8, 64)
+    assert k.append(c.cache, c.sequences, empty(2), empty(2)) is None
+    assert [x.shape for x in k.read(c.cache, c.sequences)] == [(0, 2, 64)] * 2
+    assert [x.shape for x in k.qk_norm_rope(empty(8), empty(2), torch.empty(0, dtype=torch.int32, device=gpu), rotary)] == [(0, 8, 64), (0, 2, 64)]
+    none = A.Sequences(torch.empty((0, 3), dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu), torch.empty(0, dtype=torch.int32, device=gpu), 0, 0)
+    assert k.attention(c.cache, none, empty(8), 0.1).shape == (0, 8, 64)
+    assert torch.equal(c.cache.pool, before) and k.bad_flag() == 0
