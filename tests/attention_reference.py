@@ -107,3 +107,30 @@ def attention(q, k, v, first, scale, window):
 def yarn_like(n, factor):
     f = 10000.0 ** (-torch.arange(n, dtype=torch.float64) / n)
     return f / factor, 1 + 0.1 * math.log(factor)
+
+
+def fill(pool, table_row, page_size, k, v):
+    """Writes a whole sequence, k and v [tokens][kv_heads][dim] in 64 bits, into a CPU pool, quantised."""
+    count, dim = k.shape[0], k.shape[2]
+    t = torch.arange(count)
+    page, slot = table_row[t // page_size].long(), t % page_size
+    at = 0
+    for x in (k, v):
+        codes, scales = quantise(x)
+        nibbles = codes[..., word_order(dim)]
+        for data, width in (((nibbles[..., 0::2] | nibbles[..., 1::2] << 4).to(torch.uint8), dim // 2), (scales.contiguous().view(torch.uint8), dim // 16)):
+            part = pool[:, :, at:at + page_size * width].unflatten(-1, (page_size, width))
+            part[page, :, slot] = data
+            at += page_size * width
+
+
+def marked(rows, context, dim):
+    """A sequence that tells which 32 tokens were attended to: V is 7 in dimension (t / 32) % dim and zero elsewhere, and the score of token t
+    (for a query that is 1 in dimension 0 and zero elsewhere, scale ln 2) is t / 1024 % 3 in the exponent of two.  Returns k, v [context][dim] and
+    the output [rows][dim]; all weights are powers of two and all products exact."""
+    t = torch.arange(context)
+    k, v = torch.zeros((context, dim), dtype=torch.float64), torch.zeros((context, dim), dtype=torch.float64)
+    k[:, 0], k[:, 1] = (t // 1024 % 3).double(), 7.0  # the group's scale is one
+    v[t, t // 32 % dim] = 7.0
+    weight = (t <= torch.arange(context - rows, context)[:, None]) * 2.0 ** k[:, 0]
+    return k, v, weight @ v / weight.sum(1, keepdim=True)

@@ -174,6 +174,31 @@ def test_reference_quantiser_against_a_plain_loop():
     assert torch.equal(k[0, 5], R.dequantise(codes, scales)[0]) and torch.equal(v[0, 5], R.dequantise(codes, scales)[1])
 
 
+MARKED = [(8, 2, 1, 40000), (16, 1, 1, 40000), (24, 1, 1, 20000), (8, 2, 2, 9001), (8, 1, 5, 9001), (12, 1, 4, 16001), (300, 1, 1, 5000), (16, 1, 33, 4100), (8, 2, 300, 2500),
+          (4, 1, 130, 6000), (8, 1, 200, 20011)]
+
+
+def marked_bound(want, dtype):
+    """One rounding of the output; sums of exact terms in 32 bits are far below the rest (2^-14: 2^10 additions in a row of half a step of
+    2^-23 each, should an addition truncate)."""
+    return HALF[dtype] * want + 2.0 ** -14 * want
+
+
+@pytest.mark.parametrize("heads, kv_heads, rows, context", MARKED)
+def test_the_bound_of_marked_sequences_shows_every_lost_or_doubled_tile(heads, kv_heads, rows, context):
+    k, v, want = R.marked(rows, context, 64)
+    last = min(rows, 3)  # rows at the end see every tile
+    weight = 2.0 ** k[:, 0]
+    for tile in range((context - rows) // 32):  # whole tiles that every row sees
+        here = slice(32 * tile, 32 * tile + 32)
+        part, share = weight[here] @ v[here], weight[here].sum()
+        for r in range(rows - last, rows):
+            total = weight[:context - rows + r + 1].sum()
+            for times in (-1, 1):
+                got = (want[r] * total + times * part) / (total + times * share)
+                assert ((got - want[r]).abs() > 2 * marked_bound(want[r], torch.bfloat16)).any(), tile
+
+
 # ---- GPU ----------------------------------------------------------------------------------------------------------------
 
 class Call:
@@ -912,3 +937,70 @@ def test_calls_without_rows(gpu):
     none = A.Sequences(torch.empty((0, 3), dtype=torch.int32, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu), torch.empty(0, dtype=torch.int32, device=gpu), 0, 0)
     assert k.attention(c.cache, none, empty(8), 0.1).shape == (0, 8, 64)
     assert torch.equal(c.cache.pool, before) and k.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim, page", [(64, 64), (128, 16)])
+@pytest.mark.parametrize("heads, kv_heads, rows, context", MARKED)
+def test_no_tile_of_a_split_sequence_is_lost_or_doubled(gpu, dtype, dim, page, heads, kv_heads, rows, context):
+    c = Call(gpu, [(rows, context)], heads, kv_heads, dim, page, dtype, 149)
+    k, v, want = R.marked(rows, context, dim)
+    R.fill(c.pool, c.table[0], page, *(x[:, None].expand(-1, kv_heads, -1) for x in (k, v)))
+    c.cache.pool.copy_(c.pool)
+    for scale, q in ((math.log(2), 1.0), (0.0, 3.0)):
+        c.dq[:] = 0
+        c.dq[:, :, 0] = q
+        out = c.kernels.attention(c.cache, c.sequences, c.dq, scale).cpu().double()
+        if not scale:  # all weights equal
+            seen = (torch.arange(context) <= torch.arange(context - rows, context)[:, None]).double()
+            want = seen @ v / seen.sum(1, keepdim=True)
+        assert ((out - want[:, None]).abs() <= marked_bound(want, dtype)[:, None]).all()
+    assert c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [1, 12])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_weights_of_fp16_rows_keep_their_low_bits(gpu, heads, dim):
+    """16 tokens of weight 2^-0.30005 and value 4 against 13 of weight 1 and value -4 leave 1/2600 of the terms: FP16 weights alone, the
+    first of which would be off by 0.00026, would be half of that away.  What is left: the exponential (2^-22), its argument (2^-22) and the
+    rest's own rounding (2^-22) of terms that add up to 2, then the output's."""
+    c = Call(gpu, [(1, 29)], heads, 1, dim, 16, torch.float16, 151)
+    k, v = torch.zeros((29, 1, dim), dtype=torch.float64), torch.zeros((29, 1, dim), dtype=torch.float64)
+    light = torch.arange(29) % 9 < 5
+    assert int(light.sum()) == 17
+    light[28] = False
+    k[light, 0, 0], k[:, 0, 1] = -1.0, 7.0
+    v[:] = torch.where(light, 4.0, -4.0)[:, None, None]
+    v[:, :, ::32] = 7.0  # the groups' scale is one
+    R.fill(c.pool, c.table[0], 16, k, v)
+    c.cache.pool.copy_(c.pool)
+    c.dq[:] = 0
+    c.dq[:, :, 0] = 0.3
+    weight = torch.where(light, 2.0 ** -float(torch.tensor(0.3).half()), 1.0).double()
+    want = weight @ v[:, 0] / weight.sum()
+    got = c.kernels.attention(c.cache, c.sequences, c.dq, math.log(2)).cpu().double()
+    assert want[1].abs() < 1e-3 and ((got - want).abs() <= HALF[torch.float16] * want.abs() + 7 * 4 * 2.0 ** -22).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads, kv_heads", [(8, 2), (8, 8)])
+@pytest.mark.parametrize("shapes", [
+    [(1, 9000), (512, 3000), (1, 40), (1, 17000), (1, 1)], [(1, 700)] * 40 + [(130, 130), (5, 6000)], [(40, 8000), (200, 200), (0, 50), (1, 8001), (33, 1000)]])
+def test_prompt_chunks_beside_decode_rows(gpu, heads, kv_heads, shapes):
+    """One call for rows of all kinds; every sequence tells which tokens its rows have seen."""
+    c = Call(gpu, shapes, heads, kv_heads, 64, 32, torch.bfloat16, 157, spare_rows=2)
+    wanted = []
+    for s, (n, ctx) in enumerate(shapes):
+        k, v, want = R.marked(n, ctx, 64)
+        R.fill(c.pool, c.table[s], 32, *(x[:, None].expand(-1, kv_heads, -1) for x in (k, v)))
+        wanted.append(want)
+    c.cache.pool.copy_(c.pool)
+    c.dq[:] = 0
+    c.dq[:, :, 0] = 1
+    out = torch.full((c.rows, heads, 64), 7.0, dtype=torch.bfloat16, device=gpu)
+    c.kernels.attention(c.cache, c.sequences, c.dq, math.log(2), out=out)
+    got, want = out.cpu().double(), torch.cat(wanted)
+    assert ((got[:-2] - want[:, None]).abs() <= marked_bound(want, torch.bfloat16)[:, None]).all()
+    assert (got[-2:] == 7).all() and c.kernels.bad_flag() == 0
