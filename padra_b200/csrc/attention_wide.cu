@@ -716,9 +716,9 @@ template <typename T, int D> __global__ void __launch_bounds__(kThreads, 1) Wide
                 TmemLoad16(s_address + k, y);
                 unsigned z[16];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                  const __half2 p = __hmul2(*reinterpret_cast<const __half2 *>(&y[j]), __float2half2_rn(shrink));
-                  z[j] = *reinterpret_cast<const unsigned *>(&p);
+                for (int j = 0; j < 16; ++j) { // in 32 bits: the factor may be below what FP16 holds, and the product not
+                  const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&y[j]));
+                  z[j] = Pack(p.x * shrink, p.y * shrink);
                 }
                 TmemStore16(s_address + k, z);
               }

@@ -1004,3 +1004,30 @@ def test_prompt_chunks_beside_decode_rows(gpu, heads, kv_heads, shapes):
     got, want = out.cpu().double(), torch.cat(wanted)
     assert ((got[:-2] - want[:, None]).abs() <= marked_bound(want, torch.bfloat16)[:, None]).all()
     assert (got[-2:] == 7).all() and c.kernels.bad_flag() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [1, 60, 140])
+@pytest.mark.parametrize("first", [2, 130, 258])
+def test_weights_outlast_a_large_rise_of_the_maximum(gpu, dtype, dim, rows, first):
+    """Scores (in the exponent of two) of 0, then 7 for one token, the only one with a value, then 25 for another of its tile: the value's
+    weight is 2^-18 of the largest, far above what FP16 weights lose, and everything is exact but the output's rounding.  160 equal
+    units, so that some of them lie whole in one CTA's run."""
+    c = Call(gpu, [(rows, 600)] * 20, 8, 8, dim, 64, dtype, 163)
+    k, v = torch.zeros((600, dim), dtype=torch.float64), torch.zeros((600, dim), dtype=torch.float64)
+    k[:, 4] = 7.0  # the groups' scale is one
+    k[first, 0], v[first] = 7.0, 7.0
+    k[first + 68, :4] = torch.tensor([7.0, 7.0, 7.0, 4.0])
+    for s in range(20):
+        R.fill(c.pool, c.table[s], 64, *(x[:, None].expand(-1, 8, -1) for x in (k, v)))
+    c.cache.pool.copy_(c.pool)
+    c.dq[:] = 0
+    c.dq[:, :, :4] = 1
+    out = c.kernels.attention(c.cache, c.sequences, c.dq, math.log(2)).cpu().double()
+    weight = 2.0 ** k[:, :4].sum(1)
+    for r in range(rows):
+        want = 7 * weight[first] / weight[:600 - rows + r + 1].sum()
+        assert ((out[r::rows] - want).abs() <= marked_bound(want, dtype) + (2.0 ** -25 if dtype == torch.float16 else 0)).all()
+    assert c.kernels.bad_flag() == 0
