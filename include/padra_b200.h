@@ -390,7 +390,8 @@ PADRA_API int padra_kv_read(const padra_kv_cache *cache, const padra_sequences *
 /* out = softmax(scale * q k^T) v over the cache: row at position p attends to tokens t <= p, with window > 0 only to
  * t > p - window.  q, out [rows][q_heads], q_heads a multiple of the cache's kv_heads (heads g * q_heads / kv_heads .. share KV
  * head g); out may not overlap q.  Call after the rows' own K and V have been appended.  A query that is not finite raises
- * *bad and gives zeros.  Scores are held in 32 bits: where a row's running largest score * log2(e) is
+ * *bad and gives zeros.  max_rows * q_heads / kv_heads chooses the kernel for the whole call: many decode rows are faster in a call of
+ * their own than beside a chunk.  Scores are held in 32 bits: where a row's running largest score * log2(e) is
  * beyond 2^24 in magnitude, *bad is raised and the row's output unspecified; scale * log2(e) itself has to be finite.
  * workspace: padra_attention_q4_workspace_bytes(head_dim) bytes (the same for every call), 16-byte aligned; what it holds before
  * a call does not matter.  Calls that share it, captured ones among them, must not overlap on the GPU; several host threads

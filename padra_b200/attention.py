@@ -221,7 +221,8 @@ class AttentionKernels:
         return made
 
     def attention(self, cache, sequences, q, scale, window=0, out=None, stream=None):
-        """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only."""
+        """softmax(scale q k^T) v over the cache, causal, with window > 0 over the last `window` tokens only.  The longest sequence of rows
+        chooses the kernel for all: many decode rows are faster in a call of their own than beside a chunk."""
         rows, dim, dtype, heads, at = sequences.rows, cache.head_dim, q.dtype, q.shape[1], self._here(cache, sequences)
         if out is None:
             out = _empty(q.shape, dtype, q.device, stream)

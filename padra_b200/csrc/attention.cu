@@ -13,15 +13,16 @@
 //     group, and two MMAs cover a group of 32 values, so the FP16 scale of (token, group) is applied to the group's
 //     FP32 sum.  A code becomes an FP16 number by inserting it into the mantissa of 1024 (low nibble) or 64 (high nibble), one
 //     logic operation for two codes; the offsets (1032, 72) times the query are subtracted through the accumulator's
-//     initial value.
+//     initial value, which costs some eight of its 24 bits: scores are off by about 2^-16 of sum |q k|, 2^-14 at the most.
 //   * Output: V^T is the A operand (16 values x 16 tokens).  ldmatrix.trans on 16-bit pieces hands a lane four codes of two
 //     neighbouring tokens in one register, which is where the MMA wants a pair; offset and scale are applied as FP16 (codes
 //     and offsets exact, the product rounded once, 2^-12).  Weights go from the score layout to the B operand with one 8x8
 //     transpose (movmatrix) per eight tokens.
 //   * The running maximum is only raised when a weight would pass 2^15 (weights are FP16, at least 2^8 for the largest
 //     after a raise): a warp vote per tile instead of a reduction.
-// Measured: 64 sequences of 1 to 16384 tokens, 32 heads over 4, head size 128: 81 us, 3.8 TB/s of codes and scales (58% of a copy), bound by
-// instruction issue; one sequence of 131072 tokens: 24 us and 7 us for the join; of 4097: 13 us, all latency.
+// Measured: 64 sequences of 1 to 16384 tokens, 32 heads over 4, head size 128: 81 us, 3.8 TB/s of codes and scales (58% of a copy): 168
+// registers allow 11 warps an SM, whose chains of dependent instructions fill 59% of the issue slots.  One sequence of 131072 tokens: 24 us and
+// 7 us for the join; of 4097: 13 us, all latency.
 #include <cmath>
 #include <mutex>
 #include <type_traits>
@@ -543,7 +544,8 @@ template <typename T, int D, int NT> int LaunchSplit(AttentionArgs a, int sms, c
 // Columns of a block: 8 where a sequence's rows have no more; else 16 as long as converting the codes once per block is cheaper than
 // the other kernel's blocks of 256, most of which would be empty.  Measured with 8 sequences of up to 32000 tokens and 4 KV heads, here and there:
 // heads of 128 with 32 columns 69 and 98 us, with 48 99 and 98 us (64 sequences of up to 2000: 32 columns 78 and 77 us, 48 107 and
-// 78 us); heads of 64 with 48 columns 67 and 81 us.
+// 78 us); heads of 64 with 48 columns 67 and 81 us.  One long chunk decides for the whole call: 63 decode rows beside a chunk of 512 take 414 us, in a
+// call of their own and the chunk's 162 us together.
 template <typename T, int D> int LaunchColumns(const AttentionArgs &a, int sms, cudaStream_t stream) {
   constexpr int kFewColumns = D == 64 ? 48 : 32;
   const long long columns = static_cast<long long>(a.seq.max_rows) * a.group;

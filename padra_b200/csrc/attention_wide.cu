@@ -11,13 +11,13 @@
 //   * One thread issues the MMAs: S (128 columns x 128 tokens) of each half of the block in its own tensor memory, so that one
 //     half's MMAs run under the other half's softmax.  P replaces S in tensor memory as the A operand of O += P V.
 //   * Two softmax warpgroups, one per half, one thread per column: no shuffles.  The maximum is raised lazily (by a factor of up to
-//     2^15 in FP16 weights), and only then is O rescaled.
+//     2^15 in FP16 weights), and only then are O and the weights that the tile already has rescaled (the latter rounded to FP16 a second time).
 //   * A block with at most 128 columns would leave one half idle: then the halves take even and odd tiles of the SAME columns,
 //     each with its own maximum, sum and O, and are joined through tensor memory at the end of the piece.
 // Measured (32 heads over 4, head size 128, BF16): 2048 rows behind 32767 tokens 1370 us (828 TFLOP/s), the first 2048 rows of a prompt 100 us, 5
-// rows of 8 sequences of up to 32000 tokens 98 us.  Per tile and half some 2900 cycles of softmax, 870 for S and 700 for P V; a producer warp
+// rows of 8 sequences of up to 32000 tokens 100 us.  Per tile and half some 2900 cycles of softmax, 870 for S and 700 for P V; a producer warp
 // takes 2000 to 3500 for its part of a tile.  S waits for the product that reads P, whose place it takes: 512 columns hold no second S beside
-// O of two halves, so the parts overlap between the halves only.
+// O of two halves of heads of 128 (heads of 64 keep the same places), so the parts overlap between the halves only.
 // Tensor memory: S/P of the halves in columns 0 and 128, O in 256 and 384.  Every wait is bounded in time; on expiry the CTA raises the
 // error flag and leaves.
 #include <type_traits>

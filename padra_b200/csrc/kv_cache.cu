@@ -5,7 +5,8 @@
 // that weights and the row's cos and sin stay in registers, and it has the loads of its next heads under way meanwhile, the first of them
 // from before the table is made.  cos and sin of a row are computed once per CTA for all of its heads: the angle is reduced to a
 // fraction of a turn in 64 bits, so a far position costs no precision and no slow path.
-// Bound by bandwidth for many rows (16384 rows of 32 + 4 heads of 128 in FP16: 62 us, 4.9 TB/s) and by latency for few (one row: 2.7 us).
+// Many rows (16384 of 32 + 4 heads of 128 in FP16: 64 us, 4.7 TB/s) take 73% of the copy rate at 67% of the issue slots, few (one row: 3 us)
+// are all latency.
 #include "kernels.cuh"
 #include "kv_cache.cuh"
 
@@ -492,7 +493,7 @@ __global__ void __launch_bounds__(kRowThreads) AppendKernel(KvView cache, Sequen
 }
 
 // ---- read ----
-// Bound by latency and by what the rows take to write: 12872 rows of 8 heads of 64 as FP32 in 11 us.  A warp takes one row; a lane one word (eight codes) of K and of V of one head at a time, two of each with all loads first.
+// Bound by latency (each row is looked up by itself) and by what the rows take to write: 12872 rows of 8 heads of 64 as FP32 in 11 us.  A warp takes one row; a lane one word (eight codes) of K and of V of one head at a time, two of each with all loads first.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, SequenceView seq, T *k_out, T *v_out, long long k_stride, long long v_stride,
                                                           int *bad) {
@@ -546,8 +547,8 @@ __global__ void __launch_bounds__(kRowThreads) ReadKernel(KvView cache, Sequence
     Raise(bad);
 }
 
-// Warps per row and CTAs per row: a warp takes a row whole where that fills the SMs twice over (16384 rows of 36 heads: 62 us, against
-// 69 us with two warps to a row, since fewer warps wait for tables); few rows are spread over the SMs by splitting their
+// Warps per row and CTAs per row: a warp takes a row whole where that fills the SMs twice over (16384 rows of 36 heads: 64 us, against
+// 72 us with two warps to a row, since fewer warps wait for tables); few rows are spread over the SMs by splitting their
 // heads, one unit per warp at the least.
 void Shape(int rows, int units, int *row_warps, dim3 *grid) {
   const int cta_rows = rows >= 2 * 148 * kMaxCtaRows ? kMaxCtaRows : rows >= 4 * 148 ? 4 : 1;
