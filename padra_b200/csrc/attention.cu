@@ -16,7 +16,7 @@
 //     initial value, which costs some eight of its 24 bits: scores are off by about 2^-16 of sum |q k|, 2^-14 at the most.
 //   * Output: V^T is the A operand (16 values x 16 tokens).  ldmatrix.trans on 16-bit pieces hands a lane four codes of two
 //     neighbouring tokens in one register, which is where the MMA wants a pair; offset and scale are applied as FP16 (codes
-//     and offsets exact, the product rounded once, 2^-12).  Weights go from the score layout to the B operand with one 8x8
+//     and offsets exact, the product rounded once, 2^-11).  Weights go from the score layout to the B operand with one 8x8
 //     transpose (movmatrix) per eight tokens.
 //   * The running maximum is only raised when a weight would pass 2^15 (weights are FP16, at least 2^8 for the largest
 //     after a raise): a warp vote per tile instead of a reduction.

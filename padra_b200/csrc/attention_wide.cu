@@ -5,7 +5,7 @@
 // share the KV head, so heads of a group share every K and V tile.  A tile is 128 tokens.  As in attention.cu all tiles of a call form
 // one list and every CTA (one per SM) takes an equal run of it; pieces of units are joined by JoinKernel.
 //   * Eight producer warps load codes and scales one tile ahead into registers and store FP16 rows (value = (code - 8) * scale, one
-//     rounding of 2^-12) in the 128-byte-swizzled layout, the same for K (K-major: contraction over the head's values) and V
+//     rounding of 2^-11) in the 128-byte-swizzled layout, the same for K (K-major: contraction over the head's values) and V
 //     (MN-major: contraction over tokens), so that V needs no transposition.  Values inside a block of eight lie in the order
 //     0 4 1 5 2 6 3 7 in which a code word yields pairs; Q is stored in that order and the output put back.
 //   * One thread issues the MMAs: S (128 columns x 128 tokens) of each half of the block in its own tensor memory, so that one
